@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define MI_ATTN_ABI_VERSION 12
+#define MI_ATTN_ABI_VERSION 13
 
 #if defined(__GNUC__)
 #define MI_API __attribute__((visibility("default")))
@@ -375,6 +375,42 @@ MI_API int mi_attn_cache_plan(const long long* cache_pos, const mi_decode_shape*
 MI_API int mi_attn_cache_gather(const void* k_new, const void* v_new, const void* k_cache,
                                 const void* v_cache, const int* rows, int n, void* k_out,
                                 void* v_out, const mi_decode_shape* s, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Differential attention: two softmax maps over the same values, subtracted with
+ * one learned weight per query head. The E dims of a head's q and k rows are two
+ * halves, one map each (map m, m = 1, 2):
+ *   P_m = softmax(scale q_m k_m^T + mask),  o = (P_1 - lam[h] P_2) v.
+ * No counterpart in the reference; its attention is mi_attn_fwd's.
+ *
+ *   q, o, o2, dout, dq : [B, S, H,   E]  dtype
+ *   k, v, dk, dv       : [B, S, Hkv, E]  dtype
+ *   lam, dlam          : [H]             lam_dtype
+ *   o2                 : P_2 v, which the backward reads (NULL: not written)
+ *   lse                : [2, B, H, S] float32, the natural-log logsumexp of each
+ *                        map's scaled scores (NULL: not written)
+ *   workspace          : mi_attn_diff_bwd_workspace() floats, 16-byte aligned
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int B, S, H, Hkv, E;  /* E in {32, 64, 128}; H a positive multiple of Hkv */
+  int causal;           /* 1: key j visible to query i iff j <= i; 0: every key */
+  float scale;          /* finite and > 0 */
+  int dtype;            /* mi_dtype of q, k, v, o and their gradients */
+  int lam_dtype;        /* mi_dtype of lam and dlam */
+} mi_diff_shape;
+
+MI_API int mi_attn_diff_fwd(const void* q, const void* k, const void* v, const void* lam, void* o,
+                            void* o2, float* lse, const mi_diff_shape* s, hipStream_t stream);
+
+MI_API int mi_attn_diff_bwd_workspace(const mi_diff_shape* s, long long* floats);
+
+/* Gradients of mi_attn_diff_fwd from its o, o2 and lse. No atomics: bitwise
+ * reproducible. An empty input (B, S or H of 0) writes nothing, dlam included: its
+ * gradient is zero. */
+MI_API int mi_attn_diff_bwd(const void* q, const void* k, const void* v, const void* lam,
+                            const void* o, const void* o2, const void* dout, const float* lse,
+                            float* workspace, void* dq, void* dk, void* dv, void* dlam,
+                            const mi_diff_shape* s, hipStream_t stream);
 
 /* The K extent mi_mfma_probe expects for `dtype` (16 or 2), or -1. */
 MI_API int mi_mfma_probe_k(int dtype);

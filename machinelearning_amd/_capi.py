@@ -12,7 +12,7 @@ import ctypes
 import pathlib
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libmi_attn.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 
@@ -74,10 +74,27 @@ class MiDecodeShape(ctypes.Structure):
     ]
 
 
+class MiDiffShape(ctypes.Structure):
+    """Mirror of ``mi_diff_shape``."""
+
+    _fields_ = [
+        ("B", ctypes.c_int),
+        ("S", ctypes.c_int),
+        ("H", ctypes.c_int),
+        ("Hkv", ctypes.c_int),
+        ("E", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int),
+        ("lam_dtype", ctypes.c_int),
+    ]
+
+
 _P = ctypes.c_void_p
 _SHAPE = ctypes.POINTER(MiAttnShape)
 _PSHAPE = ctypes.POINTER(MiPrologueShape)
 _DSHAPE = ctypes.POINTER(MiDecodeShape)
+_DIFF = ctypes.POINTER(MiDiffShape)
 
 # name -> (restype, argtypes); the exported surface of include/mi_attn.h.
 SIGNATURES = {
@@ -103,6 +120,9 @@ SIGNATURES = {
     "mi_attn_decode": (ctypes.c_int, [_P] * 10 + [_DSHAPE, _P]),
     "mi_attn_cache_plan": (ctypes.c_int, [_P, _DSHAPE, _P, _P, _P, _P]),
     "mi_attn_cache_gather": (ctypes.c_int, [_P] * 5 + [ctypes.c_int, _P, _P, _DSHAPE, _P]),
+    "mi_attn_diff_fwd": (ctypes.c_int, [_P] * 7 + [_DIFF, _P]),
+    "mi_attn_diff_bwd_workspace": (ctypes.c_int, [_DIFF, ctypes.POINTER(ctypes.c_longlong)]),
+    "mi_attn_diff_bwd": (ctypes.c_int, [_P] * 13 + [_DIFF, _P]),
     "mi_mfma_probe": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _P]),
     "mi_mfma_probe_k": (ctypes.c_int, [ctypes.c_int]),
     "mi_attn_error_string": (ctypes.c_char_p, [ctypes.c_int]),

@@ -1,4 +1,4 @@
-// The autograd nodes of the attention op and of the q / k prologue in C++, over
+// The autograd nodes of the attention ops and of the q / k prologue in C++, over
 // the C ABI of libmi_attn.so (include/mi_attn.h). flash_cuda.py and prologue.py
 // validate, cast and call these; the kernels' arguments, outputs and saved
 // tensors are the same as before.
@@ -222,6 +222,67 @@ struct Prologue : torch::autograd::Function<Prologue> {
   }
 };
 
+// Differential attention on contiguous [B,S,H,E] / [B,S,Hkv,E] tensors; lam [H].
+struct Diff : torch::autograd::Function<Diff> {
+  static mi_diff_shape shape(const Tensor& q, const Tensor& k, const Tensor& lam, int64_t causal,
+                             double scale) {
+    mi_diff_shape s;
+    s.B = static_cast<int>(q.size(0));
+    s.S = static_cast<int>(q.size(1));
+    s.H = static_cast<int>(q.size(2));
+    s.Hkv = static_cast<int>(k.size(2));
+    s.E = static_cast<int>(q.size(3));
+    s.causal = static_cast<int>(causal);
+    s.scale = static_cast<float>(scale);
+    s.dtype = code_of(q);
+    s.lam_dtype = code_of(lam);
+    return s;
+  }
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Tensor& lam, int64_t causal, double scale, bool keep) {
+    const c10::DeviceGuard guard(q.device());
+    const mi_diff_shape s = shape(q, k, lam, causal, scale);
+    Tensor out = at::empty_like(q), o2, lse;
+    if (keep) {   // what the backward reads
+      o2 = at::empty_like(q);
+      lse = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    }
+    check(mi_attn_diff_fwd(ptr(q), ptr(k), ptr(v), ptr(lam), ptr(out), ptr(o2), floats(lse), &s,
+                           stream_of(q)));
+    ctx->save_for_backward({q, k, v, lam, out, o2, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out;
+    {
+      at::NoGradGuard no_grad;
+      const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lam = saved[3], &o = saved[4],
+                   &o2 = saved[5], &lse = saved[6];
+      const mi_diff_shape s = shape(q, k, lam, ctx->saved_data["causal"].toInt(),
+                                    ctx->saved_data["scale"].toDouble());
+      const c10::DeviceGuard guard(q.device());
+      const Tensor dy = dense(grads[0], q.scalar_type());
+      Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+      // Nothing is written for an empty input.
+      Tensor dlam = q.numel() ? at::empty_like(lam) : at::zeros_like(lam);
+      long long n = 0;
+      check(mi_attn_diff_bwd_workspace(&s, &n));
+      const Tensor ws = at::empty({static_cast<int64_t>(n)}, lse.options());
+      check(mi_attn_diff_bwd(ptr(q), ptr(k), ptr(v), ptr(lam), ptr(o), ptr(o2), ptr(dy), floats(lse),
+                             floats(ws), ptr(dq), ptr(dk), ptr(dv), ptr(dlam), &s, stream_of(q)));
+      out = {dq, dk, dv, dlam};
+    }
+    out = once(grads, std::move(out));
+    out.resize(7);
+    return out;
+  }
+};
+
 // ---------------------------------------------------------------------------
 // Python entry points (validated by the callers)
 // ---------------------------------------------------------------------------
@@ -294,11 +355,35 @@ PyObject* py_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// diff_attn(q, k, v, lam, causal, scale) -> out.
+PyObject* py_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, lam;
+  TORCH_CHECK_TYPE(n == 6 && tensor_arg(args[0], q) && tensor_arg(args[1], k) &&
+                       tensor_arg(args[2], v) && tensor_arg(args[3], lam) && q.defined() &&
+                       k.defined() && v.defined() && lam.defined(),
+                   "diff_attn(q, k, v, lam, causal, scale)");
+  const int64_t causal = PyLong_AsLongLong(args[4]);
+  const double scale = PyFloat_AsDouble(args[5]);
+  if (PyErr_Occurred()) throw python_error();
+  const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
+                                                   v.requires_grad() || lam.requires_grad());
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = Diff::apply(q, k, v, lam, causal, scale, keep);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_attn)), METH_FASTCALL,
      "attn(q, k, v, gate, causal, window, sinks, scale, block, residual) -> (O, LSE)"},
     {"prologue", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_prologue)), METH_FASTCALL,
      "prologue(x, weight, cos, sin, eps, out_dtype) -> out"},
+    {"diff_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_diff_attn)), METH_FASTCALL,
+     "diff_attn(q, k, v, lam, causal, scale) -> out"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mi_torch", nullptr, -1, methods, nullptr, nullptr,

@@ -10,6 +10,7 @@
 
 #include "../../include/mi_attn.h"
 #include "attn_common.h"
+#include "attn_diff.h"
 
 namespace mi {
 hipError_t launch_fwd(int dtype, int D, const void* q, const void* k, const void* v, void* o,
@@ -71,6 +72,13 @@ hipError_t launch_prologue_bwd(int dtype_in, int dtype_out, int D, const void* g
                                const float* w, const float* cs, const float* sn,
                                const float* rstd, void* dx, float* dw, float* part,
                                const ProParams& p, hipStream_t st);
+long long diff_workspace_floats(const DiffParams& p);
+hipError_t launch_diff_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,
+                           void* o2, float* lse, const DiffParams& p, hipStream_t st);
+hipError_t launch_diff_bwd(int dtype, int E, const void* q, const void* k, const void* v,
+                           const void* o, const void* o2, const void* dout, const float* lse,
+                           float* ws, void* dq, void* dk, void* dv, const DiffParams& p,
+                           hipStream_t st);
 
 // One 32x32 MFMA through the same fragment helpers the attention kernels use:
 // A row l32 / B column l32 with k-slots [g*EPL, g*EPL+EPL), accumulator
@@ -776,6 +784,80 @@ int mi_attn_cache_gather(const void* k_new, const void* v_new, const void* k_cac
     return MI_ERR_ALIGN;
   return status_of(mi::launch_cache_gather(k_cache, v_cache, k_new, v_new, rows, k_out, v_out, p,
                                            stream));
+}
+
+namespace {
+
+// The attention op's own rules (validate) on the fields that the two share.
+int validate_diff(const mi_diff_shape* s) {
+  if (!s) return MI_ERR_NULL;
+  if (s->lam_dtype != MI_F32 && s->lam_dtype != MI_F16 && s->lam_dtype != MI_BF16) return MI_ERR_DTYPE;
+  const mi_attn_shape a = {s->B, s->S, s->H, s->Hkv, s->E, s->causal, 0, s->scale, s->dtype, 0, 0};
+  return validate(&a);
+}
+
+mi::DiffParams diff_params(const mi_diff_shape* s, const void* lam, void* dlam) {
+  mi::DiffParams p;
+  p.B = s->B;
+  p.S = s->S;
+  p.H = s->H;
+  p.Hkv = s->Hkv;
+  p.group = s->Hkv > 0 ? s->H / s->Hkv : 1;
+  p.causal = s->causal ? 1 : 0;
+  p.scale = s->scale;
+  p.scale_log2 = s->scale * mi::kLog2e;
+  p.resc_th = 8.f / p.scale_log2;
+  p.nblk = 0;
+  p.q_rs = (long long)s->H * s->E;
+  p.kv_rs = (long long)s->Hkv * s->E;
+  p.lam = lam;
+  p.lam_dtype = s->lam_dtype;
+  p.dlam = dlam;
+  p.div_h = mi::fast_div((unsigned)p.H);
+  p.div_hkv = mi::fast_div((unsigned)p.Hkv);
+  p.div_group = mi::fast_div((unsigned)p.group);
+  p.div_wi = mi::fast_div(1);   // set by each launcher for its grid
+  p.wi_blocks_fastest = 0;
+  return p;
+}
+
+bool empty_diff(const mi_diff_shape* s) { return s->B == 0 || s->S == 0 || s->H == 0; }
+
+}  // namespace
+
+int mi_attn_diff_fwd(const void* q, const void* k, const void* v, const void* lam, void* o, void* o2,
+                     float* lse, const mi_diff_shape* s, hipStream_t stream) {
+  const int st = validate_diff(s);
+  if (st) return st;
+  if (empty_diff(s)) return MI_OK;
+  if (!q || !k || !v || !lam || !o) return MI_ERR_NULL;
+  for (const void* t : {q, k, v, (const void*)o, (const void*)o2})
+    if (!aligned16(t)) return MI_ERR_ALIGN;
+  return status_of(mi::launch_diff_fwd(s->dtype, s->E, q, k, v, o, o2, lse,
+                                       diff_params(s, lam, nullptr), stream));
+}
+
+int mi_attn_diff_bwd_workspace(const mi_diff_shape* s, long long* floats) {
+  if (!floats) return MI_ERR_NULL;
+  const int st = validate_diff(s);
+  if (st) return st;
+  *floats = empty_diff(s) ? 0 : mi::diff_workspace_floats(diff_params(s, nullptr, nullptr));
+  return MI_OK;
+}
+
+int mi_attn_diff_bwd(const void* q, const void* k, const void* v, const void* lam, const void* o,
+                     const void* o2, const void* dout, const float* lse, float* workspace, void* dq,
+                     void* dk, void* dv, void* dlam, const mi_diff_shape* s, hipStream_t stream) {
+  const int st = validate_diff(s);
+  if (st) return st;
+  if (empty_diff(s)) return MI_OK;   // nothing written, dlam included
+  if (!q || !k || !v || !lam || !o || !o2 || !dout || !lse || !workspace || !dq || !dk || !dv || !dlam)
+    return MI_ERR_NULL;
+  for (const void* t : {q, k, v, o, o2, dout, (const void*)workspace, (const void*)dq,
+                        (const void*)dk, (const void*)dv})
+    if (!aligned16(t)) return MI_ERR_ALIGN;
+  return status_of(mi::launch_diff_bwd(s->dtype, s->E, q, k, v, o, o2, dout, lse, workspace, dq, dk,
+                                       dv, diff_params(s, lam, dlam), stream));
 }
 
 int mi_mfma_probe_k(int dtype) {

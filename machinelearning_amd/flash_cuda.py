@@ -534,6 +534,126 @@ def flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 _gate_of(gate, q, "flash_cuda.flash_attn"), block)[0]
 
 
+# ---------------------------------------------------------------------------
+# differential attention
+# ---------------------------------------------------------------------------
+def _diff_shape(q, k, lam, causal, scale):
+    B, S, H, E = q.shape
+    return _capi.MiDiffShape(B, S, H, k.shape[2], E, int(causal), scale, _DTYPE_CODE[q.dtype],
+                             _DTYPE_CODE[lam.dtype])
+
+
+def _diff_fwd(q, k, v, lam, causal, scale, keep):
+    """(out, o2, lse); o2 and lse (what the backward reads) are None unless ``keep``."""
+    B, S, H, _ = q.shape
+    out = torch.empty_like(q)
+    o2 = torch.empty_like(q) if keep else None
+    lse = torch.empty((2, B, H, S), dtype=torch.float32, device=q.device) if keep else None
+    with _on_device(q):
+        _capi.check(_capi.load().mi_attn_diff_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr(),
+            o2.data_ptr() if keep else None, lse.data_ptr() if keep else None,
+            ctypes.byref(_diff_shape(q, k, lam, causal, scale)), _stream(q)))
+    return out, o2, lse
+
+
+class _DiffAttnFn(torch.autograd.Function):
+    """Differential attention on [B,S,H,E], contiguous. ``_diff_apply`` takes the same node in
+    C++ where the call is plain eager."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, causal, scale):
+        out, o2, lse = _diff_fwd(q, k, v, lam, causal, scale, any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, lam, out, o2, lse)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, lam, out, o2, lse = ctx.saved_tensors
+        lib = _capi.load()
+        shp = ctypes.byref(_diff_shape(q, k, lam, ctx.causal, ctx.scale))
+        do = do.to(q.dtype).contiguous()
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        dlam = torch.empty_like(lam) if q.numel() else torch.zeros_like(lam)
+        n = ctypes.c_longlong(0)
+        _capi.check(lib.mi_attn_diff_bwd_workspace(shp, ctypes.byref(n)))
+        ws = torch.empty(n.value, dtype=torch.float32, device=q.device)
+        with _on_device(q):
+            _capi.check(lib.mi_attn_diff_bwd(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr(),
+                o2.data_ptr(), do.data_ptr(), lse.data_ptr(), ws.data_ptr(), dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), shp, _stream(q)))
+        return dq, dk, dv, dlam, None, None
+
+
+def _diff_apply(q, k, v, lam, causal, scale):
+    if _python_node():
+        return _DiffAttnFn.apply(q, k, v, lam, causal, scale)
+    return _ext.diff_attn(q, k, v, lam, causal, scale)
+
+
+def _lam_of(lam, q, who):
+    """The map weights as a contiguous [H] tensor on q's device (autograd-safe)."""
+    H = q.shape[2]
+    if not isinstance(lam, torch.Tensor) or lam.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"{who}: lam must be a tensor of dtype {SUPPORTED_DTYPES}, got "
+                         f"{getattr(lam, 'dtype', type(lam).__name__)}")
+    if lam.device != q.device or lam.dim() > 1 or (lam.numel() != H and lam.numel() != 1):
+        raise ValueError(f"{who}: lam must be [H] = [{H}] or one value for every head, on "
+                         f"{q.device}; got {tuple(lam.shape)} on {lam.device}")
+    return lam.reshape(-1).expand(H).contiguous()
+
+
+def _check_diff(q, k, v, scale, who):
+    """The effective dtype and the scale (default: of a half head) of a differential call."""
+    dtype = _supported_dtype(q, k, v)
+    if dtype is None or k.device != q.device or v.device != q.device:
+        raise ValueError(
+            f"{who}: unsupported inputs "
+            f"(q={tuple(q.shape)}/{q.dtype}/{q.device}, k={tuple(k.shape)}/{k.dtype}/{k.device}, "
+            f"v={tuple(v.shape)}/{v.dtype}/{v.device}); head_dim (both halves) must be one of "
+            f"{SUPPORTED_HEAD_DIMS} and the effective dtype one of {SUPPORTED_DTYPES}")
+    scale = math.sqrt(2.0 / q.shape[-1]) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{who}: scale must be finite, got {scale}")
+    return dtype, scale
+
+
+def diff_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+              scale: float | None = None, *, causal: bool = True) -> torch.Tensor:
+    """Differential attention: the difference of two softmax maps over the same values.
+
+    q [B,S,H,E], k/v [B,S,Hkv,E] -> [B,S,H,E], as ``flash_attn``, with native GQA. The E dims of
+    a head's q and k rows are two halves, one map each:
+
+        out = (softmax(scale q1 k1^T) - lam[h] softmax(scale q2 k2^T)) v
+
+    ``lam`` holds one weight per query head ([H], or one value for all of them; float32, float16
+    or bfloat16) and is differentiable, as q, k and v are. ``causal``: key j visible to query i
+    iff j <= i (else every key). ``scale`` defaults to 1/sqrt(E/2). Gradients are bitwise
+    reproducible. Under autocast q, k and v are cast as in ``flash_attn``; lam keeps its dtype.
+
+    Raises ValueError for unsupported inputs and RuntimeError when the library cannot run.
+    """
+    who = "flash_cuda.diff_attn"
+    dtype, scale = _check_diff(q, k, v, scale, who)
+    lam = _lam_of(lam, q, who)
+    if _load() is None:
+        raise RuntimeError(f"machinelearning_amd flash attention is unavailable "
+                           f"({unavailable_reason()})")
+    q, k, v = (t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+               for t in (q, k, v))
+    q, scale = _positive_scale(q, scale)
+    mma = dtype in MMA_DTYPES and _mma_ok
+    if not mma and not _f32_ok:
+        raise RuntimeError(f"float32 path unavailable ({_f32_error})")
+    if not mma and dtype != torch.float32:
+        return _diff_apply(q.float(), k.float(), v.float(), lam, bool(causal), scale).to(dtype)
+    return _diff_apply(q, k, v, lam, bool(causal), scale)
+
+
 def sdpa_reference(q, k, v, scale, causal: bool = True, window: int = 0, sinks: int = 0,
                    block: int = 0):
     """What nanolab does without the kernel: widen KV heads, transpose, SDPA.
