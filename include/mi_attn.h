@@ -91,8 +91,10 @@ typedef enum {
   MI_ERR_SCRATCH = 10,      /* mi_attn_bwd_noalloc: the shape needs more than
                                MI_ATTN_NOALLOC_SCRATCH_FLOATS of workspace */
   MI_ERR_HIP = 11,          /* a HIP runtime query failed (current device, scratch address) */
-  MI_ERR_RESIDUAL = 12      /* mi_attn_fwd_res / mi_attn_bwd_res: the output residual needs
+  MI_ERR_RESIDUAL = 12,     /* mi_attn_fwd_res / mi_attn_bwd_res: the output residual needs
                                16-bit inputs */
+  MI_ERR_TREE = 13,         /* mi_attn_step: a tree of more than MI_TREE_MAX nodes */
+  MI_ERR_MAPS = 14          /* mi_attn_step: maps not 1 or 2, or an lse of two maps */
 } mi_status;
 
 /* Size in floats of the static device array behind mi_attn_bwd_noalloc (16 MiB
@@ -411,6 +413,61 @@ MI_API int mi_attn_diff_bwd(const void* q, const void* k, const void* v, const v
                             const void* o, const void* o2, const void* dout, const float* lse,
                             float* workspace, void* dq, void* dk, void* dv, void* dlam,
                             const mi_diff_shape* s, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * A cached step whose sequences have lengths of their own and whose active block may
+ * be a tree of drafted tokens (a speculative decoder's verification), with one softmax
+ * map per head or the two of mi_attn_diff_fwd. No counterpart in the reference, whose
+ * cached step (mi_attn_decode) has one length for the batch and one chain of tokens.
+ *
+ *   q, out           : [B, T, H, D]    the T active queries (dtype)
+ *   k_new, v_new     : [B, T, Hkv, D]  the active block's keys / values
+ *   k_cache, v_cache : as in mi_attn_decode, `rows` rows per sequence and head
+ *   lens             : int32 [B], the cached rows of each sequence (clamped to
+ *                      [0, rows]; NULL: `rows`). Rows behind them are not read.
+ *   parents          : int32 [B, T], or [T] with one_tree: node t's parent, an earlier
+ *                      node of the block, or -1: the last cached token. NULL: no tree
+ *   lam              : [H] of lam_dtype, the weight of the second map (maps = 2 only)
+ *   gate             : float32 [B, T, H] output gate logits (NULL: none)
+ *   lse              : float32 [B, H, T] (maps = 1; NULL: not written)
+ *   workspace        : mi_attn_step_workspace() floats, 16-byte aligned
+ * Query t sees its sequence's cached rows and, of the block: with parents, its line of
+ * descent (itself, its parent, and so on); without, keys up to t (causal) or all T.
+ * A node whose parent is any other value, or outside the tree, is outside the tree: it
+ * is seen by nobody, its out is 0 and its lse -inf (so -2 pads shorter trees). With
+ * parents, a node whose v holds an infinity or NaN makes the rows that see it NaN and
+ * leaves the others alone; without, it reaches every row of the block.
+ * Merged in a fixed order: bitwise reproducible.
+ * ------------------------------------------------------------------------ */
+#define MI_TREE_MAX 256
+
+typedef struct {
+  int B, T, H, Hkv, D;  /* D in {32, 64, 128} (both halves, with two maps) */
+  int rows;             /* rows that a sequence's cache can hold, >= 0 */
+  int causal;           /* without parents: 1 chain, 0 every key of the block */
+  int one_tree;         /* parents is [T], for every sequence */
+  int maps;             /* 1, or 2: differential attention */
+  float scale;          /* finite and > 0 */
+  int dtype, lam_dtype;
+  long long k_batch_stride, k_head_stride;   /* cache strides in elements */
+  long long v_batch_stride, v_head_stride;
+} mi_step_shape;
+
+MI_API int mi_attn_step_workspace(const mi_step_shape* s, long long* floats);
+
+MI_API int mi_attn_step(const void* q, const void* k_new, const void* v_new, const void* k_cache,
+                        const void* v_cache, const int* lens, const int* parents, const void* lam,
+                        const float* gate, void* out, float* lse, float* workspace,
+                        const mi_step_shape* s, hipStream_t stream);
+
+/* Commit of accepted nodes: for i < count[b], row lens[b] + i of sequence b's cache (K
+ * and V, every head) becomes row path[b][i] of the block, and lens_out[b] = lens[b] +
+ * count[b]. path is int32 [B, P], count and lens_out int32 [B], lens_out not lens.
+ * Counts are clamped to [0, P] and to the room left; a node outside [0, T) copies
+ * nothing. Reads B, T, Hkv, D, rows, dtype and the strides of the shape. */
+MI_API int mi_attn_tree_commit(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                               const int* lens, const int* path, const int* count, int* lens_out,
+                               int P, const mi_step_shape* s, hipStream_t stream);
 
 /* The K extent mi_mfma_probe expects for `dtype` (16 or 2), or -1. */
 MI_API int mi_mfma_probe_k(int dtype);

@@ -15,6 +15,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "libmi_attn.so"
 ABI_VERSION = 13
 
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
+TREE_MAX = 256          # MI_TREE_MAX
 
 
 class MiAttnShape(ctypes.Structure):
@@ -74,6 +75,29 @@ class MiDecodeShape(ctypes.Structure):
     ]
 
 
+class MiStepShape(ctypes.Structure):
+    """Mirror of ``mi_step_shape``."""
+
+    _fields_ = [
+        ("B", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("H", ctypes.c_int),
+        ("Hkv", ctypes.c_int),
+        ("D", ctypes.c_int),
+        ("rows", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("one_tree", ctypes.c_int),
+        ("maps", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int),
+        ("lam_dtype", ctypes.c_int),
+        ("k_batch_stride", ctypes.c_longlong),
+        ("k_head_stride", ctypes.c_longlong),
+        ("v_batch_stride", ctypes.c_longlong),
+        ("v_head_stride", ctypes.c_longlong),
+    ]
+
+
 class MiDiffShape(ctypes.Structure):
     """Mirror of ``mi_diff_shape``."""
 
@@ -95,6 +119,7 @@ _SHAPE = ctypes.POINTER(MiAttnShape)
 _PSHAPE = ctypes.POINTER(MiPrologueShape)
 _DSHAPE = ctypes.POINTER(MiDecodeShape)
 _DIFF = ctypes.POINTER(MiDiffShape)
+_STEP = ctypes.POINTER(MiStepShape)
 
 # name -> (restype, argtypes); the exported surface of include/mi_attn.h.
 SIGNATURES = {
@@ -123,6 +148,9 @@ SIGNATURES = {
     "mi_attn_diff_fwd": (ctypes.c_int, [_P] * 7 + [_DIFF, _P]),
     "mi_attn_diff_bwd_workspace": (ctypes.c_int, [_DIFF, ctypes.POINTER(ctypes.c_longlong)]),
     "mi_attn_diff_bwd": (ctypes.c_int, [_P] * 13 + [_DIFF, _P]),
+    "mi_attn_step_workspace": (ctypes.c_int, [_STEP, ctypes.POINTER(ctypes.c_longlong)]),
+    "mi_attn_step": (ctypes.c_int, [_P] * 12 + [_STEP, _P]),
+    "mi_attn_tree_commit": (ctypes.c_int, [_P] * 8 + [ctypes.c_int, _STEP, _P]),
     "mi_mfma_probe": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _P]),
     "mi_mfma_probe_k": (ctypes.c_int, [ctypes.c_int]),
     "mi_attn_error_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -135,7 +163,8 @@ _lib = None
 # load, hipGetSymbolAddress, a launch that waits for queue space) and that are not on
 # the per-step autograd path: called through ctypes.CDLL, which releases the GIL.
 RELEASE_GIL = frozenset({"mi_attn_bwd_noalloc", "mi_attn_decode", "mi_attn_decode_workspace",
-                         "mi_attn_cache_plan", "mi_attn_cache_gather", "mi_mfma_probe",
+                         "mi_attn_cache_plan", "mi_attn_cache_gather", "mi_attn_step",
+                         "mi_attn_step_workspace", "mi_attn_tree_commit", "mi_mfma_probe",
                          "mi_mfma_probe_k"})
 
 
@@ -216,6 +245,13 @@ def decode_workspace_floats(shp: MiDecodeShape) -> int:
     """Floats of split-partial workspace a decode step needs (mi_attn_decode_workspace)."""
     n = ctypes.c_longlong(0)
     check(load().mi_attn_decode_workspace(ctypes.byref(shp), ctypes.byref(n)))
+    return int(n.value)
+
+
+def step_workspace_floats(shp: MiStepShape) -> int:
+    """Floats of split-partial workspace a step needs (mi_attn_step_workspace)."""
+    n = ctypes.c_longlong(0)
+    check(load().mi_attn_step_workspace(ctypes.byref(shp), ctypes.byref(n)))
     return int(n.value)
 
 

@@ -140,7 +140,7 @@ struct DecParams {
   const float* gate;     // [B, T, H] output gate logits (nullptr: none)
 };
 
-// Parameters of a window cache's commit (cache_commit.hip): byte strides.
+// Parameters of a cache's commit (cache_commit.hip): byte strides.
 struct CommitParams {
   int B, T, Hkv, Lc;     // batch, new rows, kv heads, cached rows
   int n;                 // rows kept per head

@@ -83,6 +83,45 @@ cache_gather_kernel(const char* __restrict__ kc, const char* __restrict__ vc,
   *reinterpret_cast<u32x4*>(dst + 16 * c) = *reinterpret_cast<const u32x4*>(src + 16 * c);
 }
 
+// Commit of a draft tree's accepted nodes: row lens[b] + i of sequence b's cache = row
+// path[b][i] of the block, i < count[b], for K and V, and lens_out = lens + count. One
+// thread per 16-byte chunk of [K | V][B][P][Hkv] rows. A node outside the block copies
+// nothing, and nothing passes the cache's end.
+__global__ void __launch_bounds__(256)
+tree_commit_kernel(const char* __restrict__ kn, const char* __restrict__ vn, char* __restrict__ kc,
+                   char* __restrict__ vc, const int* __restrict__ lens, const int* __restrict__ path,
+                   const int* __restrict__ count, int* __restrict__ lens_out, int P, int rows,
+                   CommitParams p) {
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.total) return;
+  const int c = (int)(t % p.chunks);
+  long long u = t / p.chunks;
+  const int h = (int)(u % p.Hkv);
+  u /= p.Hkv;
+  const int i = (int)(u % p.n);      // p.n = max(P, 1)
+  u /= p.n;
+  const int b = (int)(u % p.B);
+  const bool is_v = u >= p.B;
+  const int n = min(max(lens[b], 0), rows), take = min(max(count[b], 0), min(P, rows - n));
+  if (i == 0 && h == 0 && c == 0 && !is_v) lens_out[b] = n + take;
+  if (i >= take) return;
+  const int node = path[(long long)b * P + i];
+  if (node < 0 || node >= p.T) return;
+  const long long row_bytes = 16LL * p.chunks;
+  const char* src = (is_v ? vn : kn) + (((long long)b * p.T + node) * p.Hkv + h) * row_bytes;
+  char* dst = (is_v ? vc + b * p.v_sb + h * p.v_sh : kc + b * p.k_sb + h * p.k_sh) + (n + i) * row_bytes;
+  *reinterpret_cast<u32x4*>(dst + 16 * c) = *reinterpret_cast<const u32x4*>(src + 16 * c);
+}
+
+hipError_t launch_tree_commit(const void* kn, const void* vn, void* kc, void* vc, const int* lens,
+                              const int* path, const int* count, int* lens_out, int P, int rows,
+                              const CommitParams& p, hipStream_t st) {
+  hipLaunchKernelGGL(tree_commit_kernel, dim3((unsigned)((p.total + 255) / 256)), dim3(256), 0, st,
+                     (const char*)kn, (const char*)vn, (char*)kc, (char*)vc, lens, path, count,
+                     lens_out, P, rows, p);
+  return hipGetLastError();
+}
+
 hipError_t launch_cache_plan(const long long* pos, int Lc, int T, long long start, long long lo,
                              long long sinks, int* rows, long long* pos_out, int* count,
                              hipStream_t st) {

@@ -11,6 +11,7 @@
 #include "../../include/mi_attn.h"
 #include "attn_common.h"
 #include "attn_diff.h"
+#include "attn_step.h"
 
 namespace mi {
 hipError_t launch_fwd(int dtype, int D, const void* q, const void* k, const void* v, void* o,
@@ -79,6 +80,14 @@ hipError_t launch_diff_bwd(int dtype, int E, const void* q, const void* k, const
                            const void* o, const void* o2, const void* dout, const float* lse,
                            float* ws, void* dq, void* dk, void* dv, const DiffParams& p,
                            hipStream_t st);
+
+long long step_workspace_floats(int dtype, const StepParams& p, int D, bool two_maps);
+hipError_t launch_step(int dtype, int D, const void* q, const void* kc, const void* vc, const void* kn,
+                       const void* vn, void* out, float* lse, float* ws, const StepParams& p,
+                       hipStream_t st);
+hipError_t launch_tree_commit(const void* kn, const void* vn, void* kc, void* vc, const int* lens,
+                              const int* path, const int* count, int* lens_out, int P, int rows,
+                              const CommitParams& p, hipStream_t st);
 
 // One 32x32 MFMA through the same fragment helpers the attention kernels use:
 // A row l32 / B column l32 with k-slots [g*EPL, g*EPL+EPL), accumulator
@@ -240,6 +249,9 @@ const char* mi_attn_error_string(int status) {
     case MI_ERR_HIP: return "mi_attn: a HIP runtime query failed (current device / scratch address)";
     case MI_ERR_RESIDUAL:
       return "mi_attn: the output residual needs float16 / bfloat16 inputs";
+    case MI_ERR_TREE: return "mi_attn: a draft tree has at most 256 nodes (MI_TREE_MAX)";
+    case MI_ERR_MAPS:
+      return "mi_attn: maps must be 1 or 2, and two maps have no lse";
   }
   return "mi_attn: unknown status";
 }
@@ -858,6 +870,110 @@ int mi_attn_diff_bwd(const void* q, const void* k, const void* v, const void* la
     if (!aligned16(t)) return MI_ERR_ALIGN;
   return status_of(mi::launch_diff_bwd(s->dtype, s->E, q, k, v, o, o2, dout, lse, workspace, dq, dk,
                                        dv, diff_params(s, lam, dlam), stream));
+}
+
+namespace {
+
+int validate_step(const mi_step_shape* s) {
+  if (!s) return MI_ERR_NULL;
+  if (s->maps != 1 && s->maps != 2) return MI_ERR_MAPS;
+  if (s->maps == 2 && s->lam_dtype != MI_F32 && s->lam_dtype != MI_F16 && s->lam_dtype != MI_BF16)
+    return MI_ERR_DTYPE;
+  // The decode step's own rules on the fields that the two share.
+  const mi_decode_shape d = {s->B, s->T, s->H, s->Hkv, s->D, s->rows, s->rows, 0, 0, 0, s->scale, s->dtype,
+                             s->k_batch_stride, s->k_head_stride, s->v_batch_stride, s->v_head_stride};
+  const int st = validate_dec(&d);
+  if (st) return st;
+  // Query rows of a kv head and rows of the step are 32-bit in the kernels.
+  if ((long long)s->B * s->T * s->H > 0x7fffffffLL) return MI_ERR_SIZE;
+  return MI_OK;
+}
+
+mi::StepParams step_params(const mi_step_shape* s) {
+  mi::StepParams p = {};
+  p.B = s->B;
+  p.T = s->T;
+  p.H = s->H;
+  p.Hkv = s->Hkv;
+  p.rep = s->Hkv > 0 ? s->H / s->Hkv : 1;
+  p.rows = s->rows;
+  p.causal = s->causal ? 1 : 0;
+  p.scale = s->scale;
+  p.scale_log2 = s->scale * mi::kLog2e;
+  p.k_sb = s->k_batch_stride;
+  p.k_sh = s->k_head_stride;
+  p.v_sb = s->v_batch_stride;
+  p.v_sh = s->v_head_stride;
+  p.parents_sb = s->one_tree ? 0 : s->T;
+  p.lam_dtype = s->lam_dtype;
+  p.R = s->T * p.rep;
+  return p;
+}
+
+}  // namespace
+
+int mi_attn_step_workspace(const mi_step_shape* s, long long* floats) {
+  if (!floats) return MI_ERR_NULL;
+  const int st = validate_step(s);
+  if (st) return st;
+  const bool none = s->B == 0 || s->T == 0 || s->H == 0;
+  *floats = none ? 0 : mi::step_workspace_floats(s->dtype, step_params(s), s->D, s->maps == 2);
+  return MI_OK;
+}
+
+int mi_attn_step(const void* q, const void* k_new, const void* v_new, const void* k_cache,
+                 const void* v_cache, const int* lens, const int* parents, const void* lam,
+                 const float* gate, void* out, float* lse, float* workspace, const mi_step_shape* s,
+                 hipStream_t stream) {
+  const int st = validate_step(s);
+  if (st) return st;
+  if (s->maps == 2 && lse) return MI_ERR_MAPS;
+  if (parents && s->T > MI_TREE_MAX) return MI_ERR_TREE;
+  if (s->B == 0 || s->T == 0 || s->H == 0) return MI_OK;
+  if (!q || !k_new || !v_new || !out || (s->rows > 0 && (!k_cache || !v_cache)) ||
+      (s->maps == 2 && !lam))
+    return MI_ERR_NULL;
+  mi::StepParams p = step_params(s);
+  if (!workspace && mi::step_workspace_floats(s->dtype, p, s->D, s->maps == 2) > 0) return MI_ERR_NULL;
+  for (const void* t : {q, k_new, v_new, k_cache, v_cache, (const void*)out, (const void*)workspace})
+    if (!aligned16(t)) return MI_ERR_ALIGN;
+  p.lens = lens;
+  p.parents = parents;
+  p.lam = s->maps == 2 ? lam : nullptr;
+  p.gate = gate;
+  return status_of(mi::launch_step(s->dtype, s->D, q, k_cache, v_cache, k_new, v_new, out, lse,
+                                   workspace, p, stream));
+}
+
+int mi_attn_tree_commit(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                        const int* lens, const int* path, const int* count, int* lens_out, int P,
+                        const mi_step_shape* s, hipStream_t stream) {
+  const int st = validate_step(s);
+  if (st) return st;
+  if (P < 0) return MI_ERR_SHAPE;
+  if (s->B == 0) return MI_OK;
+  if (!lens || !count || !lens_out || lens_out == lens) return MI_ERR_NULL;
+  const long long elem = s->dtype == MI_F32 ? 4 : 2;
+  mi::CommitParams p = {};
+  p.B = s->B;
+  p.T = s->T;
+  p.Hkv = s->Hkv;
+  p.chunks = (int)(s->D * elem / 16);
+  // An empty path or model still sets the lengths: one row's threads, of which none copies.
+  p.n = P > 0 ? P : 1;
+  if (p.Hkv == 0) return MI_ERR_SHAPE;
+  p.total = 2LL * s->B * s->Hkv * p.n * p.chunks;
+  if ((p.total + 255) / 256 > 0x7fffffffLL) return MI_ERR_SIZE;
+  p.k_sb = s->k_batch_stride * elem;
+  p.k_sh = s->k_head_stride * elem;
+  p.v_sb = s->v_batch_stride * elem;
+  p.v_sh = s->v_head_stride * elem;
+  if (P > 0 && (!path || (s->T > 0 && (!k_new || !v_new)) || (s->rows > 0 && (!k_cache || !v_cache))))
+    return MI_ERR_NULL;
+  for (const void* t : {k_new, v_new, (const void*)k_cache, (const void*)v_cache})
+    if (!aligned16(t)) return MI_ERR_ALIGN;
+  return status_of(mi::launch_tree_commit(k_new, v_new, k_cache, v_cache, lens, path, count, lens_out,
+                                          P, s->rows, p, stream));
 }
 
 int mi_mfma_probe_k(int dtype) {

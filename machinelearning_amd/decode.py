@@ -28,6 +28,13 @@ the committed rows live in a capacity buffer, with ``cache["k"]`` a view of it.
 A commit at the end of that view writes only the block's rows, instead of
 copying the whole prefix every step.
 
+``attn_tree`` is the step of a speculative decoder: its active tokens are a tree of drafts, and
+each sequence of the batch has a cached length of its own, in ``cache["lens"]`` (int32, on the
+GPU; ``ragged_cache`` makes such a cache from one that ``attn_cached`` filled). A tree of one
+node is the ordinary decoding step of such a batch. ``tree_commit`` appends the accepted nodes.
+``diff_attn_cached`` is ``attn_cached`` for the differential attention of
+``flash_cuda.diff_attn``; ``attn_tree`` takes its ``lam`` too.
+
 Inference only: no gradient flows through the step. With autograd recording
 and an input that requires grad, this raises rather than silently dropping
 the gradient. There is no CPU fallback: without the library it raises
@@ -195,6 +202,26 @@ class _WindowCommit:
         cache["end"] = end
 
 
+def _check_block(q, k, v, who):
+    """(B, T, H, Hkv, D, effective dtype) of a step's active block, or ValueError."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4 or not t.is_cuda:
+            raise ValueError(f"{who}: {name} must be a 4-D GPU tensor, got "
+                             f"{tuple(t.shape)} on {t.device}")
+    B, T, H, D = q.shape
+    Hkv = k.shape[2]
+    if (k.shape[:2] != (B, T) or v.shape != k.shape or k.shape[3] != D or Hkv == 0
+            or H % Hkv):
+        raise ValueError(f"{who}: need q (B, T, H, D) and k, v (B, T, Hkv, D) with H a multiple "
+                         f"of Hkv, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if D not in _fc.SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"{who}: head_dim must be one of {_fc.SUPPORTED_HEAD_DIMS}, got {D}")
+    dtype = _fc.effective_dtype(q, k, v)
+    if dtype not in _fc.SUPPORTED_DTYPES:
+        raise ValueError(f"{who}: unsupported dtypes {q.dtype}/{k.dtype}/{v.dtype}")
+    return B, T, H, Hkv, D, dtype
+
+
 def attn_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, commit: bool,
                 causal: bool = False, *, window: int = 0, sinks: int = 0,
                 scale: float | None = None, gate: torch.Tensor | None = None,
@@ -216,21 +243,9 @@ def attn_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, 
     when ``return_lse``.
     """
     who = "attn_cached"
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4 or not t.is_cuda:
-            raise ValueError(f"{who}: {name} must be a 4-D GPU tensor, got "
-                             f"{tuple(t.shape)} on {t.device}")
-    B, T, H, D = q.shape
-    Hkv = k.shape[2]
-    if (k.shape[:2] != (B, T) or v.shape != k.shape or k.shape[3] != D or Hkv == 0
-            or H % Hkv):
-        raise ValueError(f"{who}: need q (B, T, H, D) and k, v (B, T, Hkv, D) with H a multiple "
-                         f"of Hkv, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if D not in _fc.SUPPORTED_HEAD_DIMS:
-        raise ValueError(f"{who}: head_dim must be one of {_fc.SUPPORTED_HEAD_DIMS}, got {D}")
-    dtype = _fc.effective_dtype(q, k, v)
-    if dtype not in _fc.SUPPORTED_DTYPES:
-        raise ValueError(f"{who}: unsupported dtypes {q.dtype}/{k.dtype}/{v.dtype}")
+    B, T, H, Hkv, D, dtype = _check_block(q, k, v, who)
+    if "lens" in cache:
+        raise ValueError(f"{who}: the cache holds a length for each sequence ('lens'): attn_tree's")
     window, sinks = int(window or 0), int(sinks or 0)
     if window < 0:
         raise ValueError(f"{who}: window must be >= 0, got {window}")
@@ -318,3 +333,245 @@ def attn_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, 
         _commit_append(cache, "k", _KBUF, ck, kt, Lc, T)
         _commit_append(cache, "v", _VBUF, cv, vt, Lc, T)
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# steps over sequences of different lengths: draft trees, differential attention
+# ---------------------------------------------------------------------------
+_STEPS: dict = {}
+
+
+def _step_shape(key: tuple):
+    """(struct, byref pointer, workspace floats) of a step's shape, as ``_shape``."""
+    hit = _STEPS.get(key)
+    if hit is None:
+        shp = _capi.MiStepShape(*key)
+        hit = (shp, ctypes.byref(shp), _capi.step_workspace_floats(shp))
+        if len(_STEPS) >= _SHAPES_MAX:
+            _STEPS.clear()
+        _STEPS[key] = hit
+    return hit
+
+
+def _step_workspace(dev, stream, floats):
+    """The stream's workspace, or under graph capture one of the graph's own: two graphs that
+    share one may be replayed side by side, and outlive its place in the list."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(floats, dtype=torch.float32, device=dev)
+    return _workspace(dev, stream, floats)
+
+
+def _refuse_grad(who, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who}: the cached step is inference-only (no backward); call it "
+                           f"under torch.no_grad() or with detached inputs")
+
+
+def _whole_numbers(t, shapes, dev, who, name, top):
+    """An int32 contiguous copy of ``t`` where it is not one already; values that int32 cannot
+    hold keep their side of [0, top]."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{who}: {name} must be an int32 or int64 tensor, got "
+                         f"{getattr(t, 'dtype', type(t).__name__)}")
+    if t.device != dev or tuple(t.shape) not in shapes:
+        raise ValueError(f"{who}: {name} must be {' or '.join(map(str, shapes))} on {dev}, got "
+                         f"{tuple(t.shape)} on {t.device}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-2, top + 1).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _step(who, q, k, v, dims, cache, parents, causal, lam, scale, gate, return_lse):
+    """One launch of ``mi_attn_step`` over ``cache``; q, k, v as the caller gave them."""
+    B, T, H, Hkv, D, dtype = dims
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"{who}: q, k and v must be on one device, got {dev}, {k.device}, {v.device}")
+    scale = math.sqrt((1 if lam is None else 2) / D) if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"{who}: scale must be finite and > 0, got {scale}")
+    if lam is not None:
+        lam = _fc._lam_of(lam, q, who)
+        if return_lse:
+            raise ValueError(f"{who}: two maps have no lse")
+    ck, cv = cache.get("k"), cache.get("v")
+    if (ck is None) != (cv is None):
+        raise ValueError(f"{who}: cache holds only one of 'k' / 'v'")
+    rows = 0 if ck is None else int(ck.shape[2])
+    strides = (0, 0, 0, 0)
+    if ck is not None:
+        ck = _cache_tensor(ck, B, Hkv, D, dtype, dev, who, "k")
+        cv = _cache_tensor(cv, B, Hkv, D, dtype, dev, who, "v")
+        if cv.shape[2] != rows:
+            raise ValueError(f"{who}: cache 'k' and 'v' lengths differ: {rows} vs {cv.shape[2]}")
+        strides = (ck.stride(0), ck.stride(1), cv.stride(0), cv.stride(1))
+    lens = cache.get("lens")
+    if lens is not None:
+        lens = _whole_numbers(lens, ((B,),), dev, who, "cache['lens']", rows)
+    one_tree = 0
+    if parents is not None:
+        parents = _whole_numbers(parents, ((T,), (B, T)), dev, who, "parents", T)
+        if T > _capi.TREE_MAX:
+            raise ValueError(f"{who}: a tree has at most {_capi.TREE_MAX} nodes, got {T}")
+        one_tree = int(parents.dim() == 1)
+    if gate is not None:
+        if tuple(gate.shape) == (B, T, H, 1):
+            gate = gate.squeeze(-1)
+        if tuple(gate.shape) != (B, T, H):
+            raise ValueError(f"{who}: gate logits must be (B, T, H) = {(B, T, H)}, got "
+                             f"{tuple(gate.shape)}")
+        gate = gate.to(device=dev, dtype=torch.float32).contiguous()
+    _refuse_grad(who, q, k, v, lam, gate)
+    if _fc._load() is None:
+        raise RuntimeError(f"{who}: the library is unavailable ({_fc.unavailable_reason()})")
+    q, k, v = (_dense(t, dtype) for t in (q, k, v))
+    out = torch.empty_like(q)
+    lse = torch.empty(B, H, T, dtype=torch.float32, device=dev) if return_lse else None
+    _, shp, nws = _step_shape((B, T, H, Hkv, D, rows, int(causal), one_tree, 1 if lam is None else 2,
+                               scale, _fc._DTYPE_CODE[dtype],
+                               0 if lam is None else _fc._DTYPE_CODE[lam.dtype]) + strides)
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+    with _fc._on_device(q):
+        stream = _fc._stream(q)
+        ws = _step_workspace(dev, stream, nws) if nws else None
+        _capi.check(_capi.load().mi_attn_step(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(ck), ptr(cv), ptr(lens), ptr(parents),
+            ptr(lam), ptr(gate), out.data_ptr(), ptr(lse), ptr(ws), shp, stream))
+    return (out, lse) if return_lse else out
+
+
+def attn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict,
+              parents: torch.Tensor, *, lam: torch.Tensor | None = None,
+              scale: float | None = None, gate: torch.Tensor | None = None,
+              return_lse: bool = False):
+    """Attention of a tree of drafted tokens over each sequence's cache.
+
+    q (B, T, H, D), k / v (B, T, Hkv, D): the T <= 256 drafted tokens, rotated for their depth.
+    ``parents`` (B, T), or (T,) for one tree in every sequence, int32 or int64: node t's parent
+    is an earlier node of the tree, or -1 for the last cached token. Node t sees its sequence's
+    cached rows, itself and its ancestors. A node with any other parent (-2 pads shorter trees),
+    and every node under it, is outside the tree: its output is 0 and nobody sees it. A node
+    whose v holds an infinity or NaN makes the rows that see it NaN and leaves the others alone.
+
+    ``cache`` is ``attn_cached``'s dict (every row of ``cache["k"]`` counts), or one with
+    ``cache["lens"]`` (B,), the rows that count in each sequence; what lies behind them is not
+    read. Nothing is committed: ``tree_commit`` does that once the nodes are verified.
+
+    ``lam``: the two maps of ``flash_cuda.diff_attn``, subtracted with these weights (``scale``
+    then defaults to 1/sqrt(D/2)). ``gate`` as in ``attn_cached``. Returns the (B, T, H, D)
+    output, and the (B, H, T) float32 LSE too when ``return_lse`` (one map only).
+    """
+    who = "attn_tree"
+    dims = _check_block(q, k, v, who)
+    if "pos" in cache:
+        raise ValueError(f"{who}: a windowed cache ('pos') holds no draft trees")
+    return _step(who, q, k, v, dims, cache, parents, True, lam, scale, gate, return_lse)
+
+
+def diff_attn_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                     cache: dict, commit: bool, causal: bool = False, *,
+                     scale: float | None = None, gate: torch.Tensor | None = None) -> torch.Tensor:
+    """``attn_cached`` for differential attention (``flash_cuda.diff_attn``): the same cache dict,
+    block masks and commit, without a window. q (B, T, H, E), k / v (B, T, Hkv, E), ``lam`` (H,)
+    or one value; ``scale`` defaults to 1/sqrt(E/2). Returns the (B, T, H, E) output.
+    """
+    who = "diff_attn_cached"
+    dims = _check_block(q, k, v, who)
+    for name in ("lens", "pos"):
+        if name in cache:
+            raise ValueError(f"{who}: the cache holds {name!r}: "
+                             + ("a length for each sequence, attn_tree's" if name == "lens"
+                                else "a window's, which differential attention has not"))
+    out = _step(who, q, k, v, dims, cache, None, causal, lam, scale, gate, False)
+    if commit:
+        T, dtype, dev = dims[1], dims[5], q.device
+        for name, held, new in (("k", _KBUF, k), ("v", _VBUF, v)):
+            old = cache.get(name)
+            if old is not None:
+                old = _cache_tensor(old, dims[0], dims[3], dims[4], dtype, dev, who, name)
+            _commit_append(cache, name, held, old, _dense(new, dtype).transpose(1, 2),
+                           0 if old is None else old.shape[2], T)
+    return out
+
+
+def ragged_cache(cache: dict, rows: int, lens: torch.Tensor | None = None) -> dict:
+    """A cache for ``attn_tree`` and ``tree_commit`` from one that ``attn_cached`` (or
+    ``diff_attn_cached``) filled: ``"k"`` and ``"v"`` with room for ``rows`` rows per sequence,
+    and ``"lens"`` (B,) int32, how many of them count (all that the old cache holds, unless
+    ``lens`` gives fewer). The old cache is left alone.
+    """
+    who = "ragged_cache"
+    ck, cv = cache.get("k"), cache.get("v")
+    if ck is None or cv is None or "pos" in cache or "lens" in cache:
+        raise ValueError(f"{who}: needs a cache of attn_cached without a window")
+    B, Hkv, L, D = ck.shape
+    if cv.shape != ck.shape or rows < L:
+        raise ValueError(f"{who}: rows must be at least the {L} that the cache holds, and 'k' and "
+                         f"'v' alike: got {rows}, {tuple(ck.shape)}, {tuple(cv.shape)}")
+    if lens is None:
+        lens = torch.full((B,), L, dtype=torch.int32, device=ck.device)
+    else:
+        lens = _whole_numbers(lens, ((B,),), ck.device, who, "lens", L).clamp(0, L)
+    new = {"lens": lens}
+    for name, old in (("k", ck), ("v", cv)):
+        new[name] = torch.empty(B, Hkv, rows, D, dtype=old.dtype, device=old.device)
+        new[name][:, :, :L].copy_(old)
+    return new
+
+
+def tree_commit(k: torch.Tensor, v: torch.Tensor, cache: dict, path: torch.Tensor,
+                count: torch.Tensor) -> None:
+    """Append the accepted nodes of a draft tree to each sequence's cache.
+
+    k / v (B, T, Hkv, D) are the tree's, as ``attn_tree`` took them. ``path`` (B, P) lists each
+    sequence's accepted nodes in order and ``count`` (B,) says how many of them count (int32 or
+    int64, on the GPU: nothing waits for the host). Row ``lens[b] + i`` of ``cache["k"]`` and
+    ``cache["v"]`` becomes that of node ``path[b, i]``, in place, and ``cache["lens"]`` a new
+    tensor, ``lens + count``: a shallow copy of the dict made before keeps its lengths. A graph
+    that is captured with this call copies the new lengths back itself.
+
+    The caches need room for the accepted rows: lengths stop at ``cache["k"].shape[2]``, and rows
+    past it are dropped. A node outside [0, T) leaves its row as it was.
+    """
+    who = "tree_commit"
+    B, T, _, Hkv, D, dtype = _check_block(k, k, v, who)
+    dev = k.device
+    for name in ("k", "v"):
+        t = cache.get(name)
+        if t is None or t.dim() != 4 or tuple(t.shape[:2]) != (B, Hkv) or t.shape[3] != D:
+            raise ValueError(f"{who}: cache[{name!r}] must be (B, Hkv, rows, D) = ({B}, {Hkv}, rows, "
+                             f"{D}), got {None if t is None else tuple(t.shape)}")
+        # Rows are written in place, so a cache that would have to be copied is refused.
+        chunk = 16 // t.element_size()
+        if (t.dtype != dtype or t.device != dev or t.stride(3) != 1 or t.stride(2) != D
+                or t.stride(0) % chunk or t.stride(1) % chunk or t.data_ptr() % 16):
+            raise ValueError(f"{who}: cache[{name!r}] must be {dtype} on {dev} with rows {D} apart, "
+                             f"16-byte aligned; got {t.dtype} on {t.device}, strides {t.stride()}")
+    ck, cv = cache["k"], cache["v"]
+    rows = int(ck.shape[2])
+    if cv.shape[2] != rows:
+        raise ValueError(f"{who}: cache 'k' and 'v' lengths differ: {rows} vs {cv.shape[2]}")
+    if v.device != dev:
+        raise ValueError(f"{who}: k and v must be on one device, got {dev}, {v.device}")
+    if "lens" not in cache:
+        raise ValueError(f"{who}: the cache has no 'lens' (see ragged_cache)")
+    lens = _whole_numbers(cache["lens"], ((B,),), dev, who, "cache['lens']", rows)
+    if not isinstance(path, torch.Tensor) or path.dim() != 2:
+        raise ValueError(f"{who}: path must be (B, P), got {tuple(getattr(path, 'shape', ()))}")
+    P = int(path.shape[1])
+    path = _whole_numbers(path, ((B, P),), dev, who, "path", T)
+    count = _whole_numbers(count, ((B,),), dev, who, "count", P)
+    _refuse_grad(who, k, v)
+    if _fc._load() is None:
+        raise RuntimeError(f"{who}: the library is unavailable ({_fc.unavailable_reason()})")
+    k, v = _dense(k, dtype), _dense(v, dtype)
+    new = torch.empty(B, dtype=torch.int32, device=dev)
+    _, shp, _ = _step_shape((B, T, Hkv, Hkv, D, rows, 1, 0, 1, 1.0, _fc._DTYPE_CODE[dtype], 0,
+                             ck.stride(0), ck.stride(1), cv.stride(0), cv.stride(1)))
+    with _fc._on_device(k):
+        _capi.check(_capi.load().mi_attn_tree_commit(
+            k.data_ptr(), v.data_ptr(), ck.data_ptr(), cv.data_ptr(), lens.data_ptr(),
+            path.data_ptr(), count.data_ptr(), new.data_ptr(), P, shp, _fc._stream(k)))
+    cache["lens"] = new

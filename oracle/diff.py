@@ -2,8 +2,9 @@
 
     P_m = softmax(scale * q_m k_m^T + mask),  out = (P_1 - lam_h P_2) v
 
-on q [B,T,H,E], k/v [B,L,Hkv,E] (the halves m of the E dims of q and k), lam [H]. Query t may
-see key j where ``keep`` [T, L] says so. Also bounds on what roundings do to each result, for
+on q [B,T,H,E], k/v [B,L,Hkv,E] (the halves m of the E dims of q and k), lam [H]; with lam None,
+ordinary attention: one map of all E dims. Query t may see key j where ``keep`` [T, L] says so,
+and sees one at least. Also bounds on what roundings do to each result, for
 the tolerances of the tests.
 """
 
@@ -39,7 +40,7 @@ class Case:
     q: torch.Tensor
     k: torch.Tensor
     v: torch.Tensor
-    lam: torch.Tensor
+    lam: torch.Tensor | None
     scale: float
     keep: torch.Tensor
 
@@ -47,9 +48,11 @@ class Case:
         H, E = self.q.shape[2], self.q.shape[3]
         self.H, self.Hkv, self.E = H, self.k.shape[2], E
         self.qh, self.kh, self.vh = (_heads(t, H) for t in (self.q, self.k, self.v))
-        self.w = (torch.ones(1, 1, 1, 1, dtype=torch.float64),
-                  -self.lam.detach().cpu().double().reshape(1, H, 1, 1))
-        self.half = (slice(0, E // 2), slice(E // 2, E))
+        self.w = (torch.ones(1, 1, 1, 1, dtype=torch.float64),)
+        self.half = (slice(0, E),)
+        if self.lam is not None:
+            self.w += (-self.lam.detach().cpu().double().reshape(1, H, 1, 1),)
+            self.half = (slice(0, E // 2), slice(E // 2, E))
         self.P, self.lse = [], []
         for m in self.half:
             s = self.scale * self.qh[..., m] @ self.kh[..., m].transpose(-1, -2)
@@ -81,12 +84,12 @@ class Case:
     # the other types reach 2^-126). Sums are taken in float32.
     def _slack(self) -> float:
         """Relative error of a P, and of a sum of products, in float32: the scores' own
-        (E / 2 products, then a few units of the largest score's exponent) and the length
+        (at most E products, then a few units of the largest score's exponent) and the length
         of the sums."""
         f = 2.0 ** -24
         big = max(float((abs(self.scale) * self.qh[..., m].abs() @ self.kh[..., m].abs().transpose(-1, -2))
                         .max()) for m in self.half) if self.qh.numel() and self.kh.numel() else 0.0
-        return f * (self.E / 2 * big + 4 * big + 64 + self.E + self.keep.shape[0] + self.keep.shape[1])
+        return f * (self.E * big + 4 * big + 64 + self.E + self.keep.shape[0] + self.keep.shape[1])
 
     def _value_bounds(self, u, tiny):
         """|error| of P_m v before it is rounded, from P's rounding and float32. (The forward
@@ -98,6 +101,11 @@ class Case:
     def out_bound(self, u: float, tiny: float = 0.0) -> torch.Tensor:
         e = sum(w.abs() * b for w, b in zip(self.w, self._value_bounds(u, tiny)))
         return (e + u * (self.out().transpose(1, 2).abs() + e) + tiny).transpose(1, 2)
+
+    def lse_bound(self) -> torch.Tensor:
+        """|error| of a map's LSE: its scores' absolute error and its sum's relative one, and
+        its own rounding."""
+        return self._slack() + 2.0 ** -23 * self.lse[0].abs()
 
     def grad_bounds(self, do: torch.Tensor, u: float, tiny: float = 0.0):
         a = do.detach().cpu().double().transpose(1, 2)
