@@ -26,7 +26,9 @@ struct StepParams {
   const void* lam;                     // [H] map weights (two maps only)
   int lam_dtype;
   int R;                               // query rows per kv head: T * rep
-  int nsplit;                          // key splits of a unit
+  int nsplit;                          // key splits of a unit (16-bit: workgroups in all)
+  int min_blocks;                      // 16-bit: key blocks that a workgroup takes at least
+  float resc_th;                       // 16-bit: lazy-rescale threshold in raw score units
 };
 
 constexpr int kTreeMax = 256;          // nodes of a tree: one per thread of a workgroup

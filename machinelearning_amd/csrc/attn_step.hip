@@ -1,4 +1,4 @@
-// The cached step of attn_step.h for every dtype: keys split over workgroups, one running
+// The cached step of attn_step.h for float32: keys split over workgroups, one running
 // softmax per query row and map, partials merged in split order (bitwise reproducible).
 //
 // A workgroup of four waves walks a range of key blocks of one (batch, kv head). Its
@@ -287,7 +287,7 @@ hipError_t step_t(const void* q, const void* kc, const void* vc, const void* kn,
 }
 
 template <typename F>
-hipError_t by_type(int dtype, int D, bool two_maps, F f) {
+hipError_t by_shape(int D, bool two_maps, F f) {
   const auto by_maps = [&](auto t, auto d) {
     return two_maps ? f(t, d, std::integral_constant<int, 2>{}) : f(t, d, std::integral_constant<int, 1>{});
   };
@@ -299,17 +299,18 @@ hipError_t by_type(int dtype, int D, bool two_maps, F f) {
     }
     return hipErrorInvalidValue;
   };
-  switch (dtype) {
-    case 0: return by_dim(float{});
-    case 1: return by_dim(_Float16{});
-    case 2: return by_dim(__bf16{});
-  }
-  return hipErrorInvalidValue;
+  return by_dim(float{});
 }
 
 }  // namespace
 
+long long step16_workspace_floats(const StepParams& p, int D, bool two_maps);
+hipError_t launch_step16(int dtype, int D, const void* q, const void* kc, const void* vc, const void* kn,
+                         const void* vn, void* out, float* lse, float* ws, const StepParams& p,
+                         hipStream_t st);
+
 long long step_workspace_floats(int dtype, const StepParams& p, int D, bool two_maps) {
+  if (dtype != 0) return step16_workspace_floats(p, D, two_maps);
   const int maps = two_maps ? 2 : 1;
   const long long splits = p.R <= 32 ? 4LL * step_splits<4>(p) : step_splits<1>(p);
   return (long long)p.B * p.Hkv * p.R * splits * (maps * D + 2 * maps);
@@ -318,7 +319,8 @@ long long step_workspace_floats(int dtype, const StepParams& p, int D, bool two_
 hipError_t launch_step(int dtype, int D, const void* q, const void* kc, const void* vc, const void* kn,
                        const void* vn, void* out, float* lse, float* ws, const StepParams& p,
                        hipStream_t st) {
-  return by_type(dtype, D, p.lam != nullptr, [&](auto t, auto d, auto m) {
+  if (dtype != 0) return launch_step16(dtype, D, q, kc, vc, kn, vn, out, lse, ws, p, st);
+  return by_shape(D, p.lam != nullptr, [&](auto t, auto d, auto m) {
     using T = decltype(t);
     constexpr int DD = decltype(d)::value, MM = decltype(m)::value;
     return p.R <= 32 ? step_t<T, DD, MM, 4>(q, kc, vc, kn, vn, out, lse, ws, p, st)

@@ -1,0 +1,608 @@
+// The cached step of attn_step.h for 16-bit inputs: MFMA tiles fed by LDS-DMA, the keys of
+// the whole batch dealt evenly to the workgroups.
+//
+//  * Work. A unit is one (sequence, kv head, group of NR row tiles of 32 query rows); its
+//    key blocks, unit after unit, form one line of N blocks, cut into equal pieces, one per
+//    workgroup: sequences of any lengths load the chip evenly. (Cut per sequence, the
+//    longest one sets the time.) The lengths are on the GPU, so each workgroup finds its
+//    piece itself, from a prefix sum over them. A piece is one or more fragments of units;
+//    a unit that one fragment covers is written at once, the others' fragments go to the
+//    workspace as float32 partials (at most the first and the last of a piece are partial:
+//    two slots per workgroup) and step16_combine_kernel merges them in order.
+//  * Waves. NR row waves x NK key waves: up to 32 rows, each of four waves takes every
+//    fourth block (its own LDS ring, no barrier in the loop); with more rows, waves share
+//    the blocks of a ring. A wave's scores are transposed, S^T = K Q^T, so a lane owns a
+//    query row and P^T feeds O^T += V^T P^T from registers (attn16.h's tiles).
+//  * Masks only where a block needs one: a sequence's last cached block (rows past it read
+//    as zeros through the buffer's bound) and the active block's, one word per block.
+#include <type_traits>
+
+#include "attn16.h"
+#include "attn_diff.h"
+#include "attn_step.h"
+
+namespace mi {
+
+namespace {
+
+template <int D, int MAPS, int NR, int NK>
+struct Step16 {
+  static constexpr int W = NR * NK;              // waves
+  static constexpr int CH = D / 8;               // 16-byte chunks per row
+  static constexpr int TILE = 32 * D * 2;        // K (or V) of a block
+  static constexpr int LD = TILE / 1024;         // DMA instructions per tile
+  static constexpr int IPW = 2 * LD >= NR ? 2 * LD / NR : 1;   // ... of K and V per wave
+  static constexpr int NS = NK == 4 ? 2 : 3;     // ring stages
+  static constexpr int RING = NK * NS * 2 * TILE;
+  // Key waves' float32 results, merged in LDS (the ring's bytes, after the loop).
+  static constexpr int MERGE = NK > 1 ? W * 32 * MAPS * D * 4 : 0;
+  static constexpr int LDS = RING > MERGE ? RING : MERGE;
+  static constexpr int DS = D / 16, DM = DS / MAPS, DT = D / 32;
+  // A slot: the rows' O of each map, then their (m, l).
+  static constexpr int ROWS = NR * 32, SLOT = ROWS * (MAPS * D + 2 * MAPS);
+};
+
+// The line of blocks: N of them, `per` to a workgroup.
+struct Line {
+  long long N, per;
+};
+
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  const unsigned lo = (unsigned)uniform((int)x), hi = (unsigned)uniform((int)(x >> 32));
+  return (long long)((unsigned long long)hi << 32 | lo);
+}
+
+__device__ __forceinline__ int step_blocks(const StepParams& p, int b) {
+  return (step_len(p, b) + 31) / 32 + (p.T + 31) / 32;
+}
+
+// Blocks of the sequences before `b` (each counted once), all lanes of a wave.
+__device__ __forceinline__ long long blocks_before(const StepParams& p, int b) {
+  long long sum = 0;
+  for (int i = threadIdx.x & 63; i < b; i += 64) sum += step_blocks(p, i);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  return uniform(sum);
+}
+
+__device__ __forceinline__ Line step_line(const StepParams& p, int units_per_seq) {
+  const long long N = blocks_before(p, p.B) * units_per_seq;
+  const long long per = (N + p.nsplit - 1) / p.nsplit;
+  return {N, per > p.min_blocks ? per : p.min_blocks};
+}
+
+// The sequence that holds block x (x < N / units) of the sequences' blocks counted once,
+// and the blocks before it: a wave's scan, 64 sequences a round.
+__device__ __forceinline__ int find_seq(const StepParams& p, long long x, long long& before) {
+  const int lane = threadIdx.x & 63;
+  before = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int own = b0 + lane < p.B ? step_blocks(p, b0 + lane) : 0;
+    long long upto = own;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const long long y = __shfl_up(upto, s);
+      if (lane >= s) upto += y;
+    }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + upto > x);
+    if (past || b0 + 64 >= p.B) {
+      const int l = past ? __builtin_ctzll(past) : min(63, p.B - 1 - b0);
+      before += uniform(__shfl(upto - own, l));
+      return b0 + l;
+    }
+    before += uniform(__shfl(upto, 63));
+  }
+}
+
+// A tree of at most 64 nodes in a wave's registers: lane t holds node t's line of descent
+// and whether it is in the tree (tree_build's doubling, without LDS or barriers).
+struct WaveTree {
+  unsigned lo, hi;
+  int up;
+};
+__device__ __forceinline__ WaveTree wave_tree(const StepParams& p, int b) {
+  const int t = threadIdx.x & 63;
+  WaveTree w;
+  w.lo = t < 32 ? 1u << t : 0u;
+  w.hi = t < 32 ? 0u : 1u << (t - 32);
+  w.up = -2;
+  if (t < p.T) {
+    const int x = p.parents[(long long)b * p.parents_sb + t];
+    if (x >= -1 && x < t) w.up = x;
+  }
+  while (__builtin_amdgcn_ballot_w64(w.up >= 0)) {
+    const int from = w.up >= 0 ? w.up : t;
+    const unsigned lo = __shfl(w.lo, from), hi = __shfl(w.hi, from);
+    const int up = __shfl(w.up, from);
+    w.lo |= lo;
+    w.hi |= hi;
+    w.up = up;
+  }
+  return w;
+}
+
+template <typename T, int D, int MAPS>
+__device__ __forceinline__ void step16_emit(const StepParams& p, T* __restrict__ out, float* __restrict__ lse,
+                                            int b, int kvh, int r, int d0, const f32x4 (&o)[MAPS],
+                                            const float (&M)[MAPS], const float (&L)[MAPS], bool dead,
+                                            bool poisoned) {
+  const int t = r / p.rep, h = kvh * p.rep + r % p.rep;
+  f32x4 y = o[0] * (1.f / L[0]);
+  if constexpr (MAPS == 2) y -= o[1] * (load_as_float(p.lam, p.lam_dtype, h) / L[1]);
+  if (p.gate) y *= 1.f / (1.f + __expf(-p.gate[((long long)b * p.T + t) * p.H + h]));
+  if (poisoned) y = f32x4{NAN, NAN, NAN, NAN};
+  if (dead) y = f32x4{0.f, 0.f, 0.f, 0.f};
+  st_quad<T>(out + (((long long)b * p.T + t) * p.H + h) * D + d0, y[0], y[1], y[2], y[3]);
+  if (lse && d0 == 0)
+    lse[((long long)b * p.H + h) * p.T + t] = dead ? -INFINITY : poisoned ? NAN : M[0] * p.scale + logf(L[0]);
+}
+
+}  // namespace
+
+template <typename T, int D, int MAPS, int NR, int NK, bool TREE>
+__global__ void __launch_bounds__(64 * NR * NK)
+step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __restrict__ Vc,
+              const T* __restrict__ Kn, const T* __restrict__ Vn, T* __restrict__ O,
+              float* __restrict__ LSE, float* __restrict__ part, StepParams p) {
+  using C = Step16<D, MAPS, NR, NK>;
+  using M = Mfma32<T>;
+  using frag = typename M::frag;
+  constexpr int NS = C::NS, DS = C::DS, DM = C::DM, DT = C::DT, TILE = C::TILE, NT = 64 * C::W;
+  static_assert(NT >= kTreeMax, "tree_build wants a thread per node");
+  __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+  __shared__ float ml[NK > 1 ? C::W : 1][32][2 * MAPS];
+  __shared__ TreeLds tree;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, g = lane >> 5;
+  const int rw = wave % NR, kw = wave / NR;
+  const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;   // units per sequence
+  const Line line = step_line(p, ups);
+  long long at = (long long)blockIdx.x * line.per;
+  const long long end = at + line.per < line.N ? at + line.per : line.N;
+  if (at >= end) return;
+
+  char* ring = lds + kw * (NS * 2 * TILE);
+  int kaddr[DS];
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) kaddr[ds] = tile_off<D>(l32, 2 * ds + g);
+  int vaddr[DT][2];
+  {
+    const int G = lane >> 4, m = lane & 15, row = 4 * (G >> 1) + (m >> 2);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int col = dt * 32 + 16 * (G & 1) + 4 * (m & 3);
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) vaddr[dt][hh] = tile_off<D>(row + 8 * hh, col >> 3) + (col & 7) * 2;
+    }
+  }
+  const float c = p.scale_log2;
+  const bool small_tree = TREE && p.T <= 64;
+
+  long long before;                       // blocks of earlier sequences, counted once
+  int b = find_seq(p, at / ups, before);
+  while (true) {
+    // The fragment [at, stop) of unit u of sequence b.
+    const int Lc = step_len(p, b), ncb = (Lc + 31) / 32, nb = ncb + (p.T + 31) / 32;
+    const long long in_seq = at - before * ups;
+    const int u = (int)(in_seq / nb), blk0 = (int)(in_seq - (long long)u * nb);
+    const int blk1 = (int)min((long long)nb, blk0 + (end - at));
+    const int kvh = u / ngrp, grp = u % ngrp;
+    const bool whole = blk0 == 0 && blk1 == nb, has_tail = blk1 > ncb;
+
+    const char* kc = reinterpret_cast<const char*>(Kc + (long long)b * p.k_sb + (long long)kvh * p.k_sh);
+    const char* vc = reinterpret_cast<const char*>(Vc + (long long)b * p.v_sb + (long long)kvh * p.v_sh);
+    const char* kn = reinterpret_cast<const char*>(Kn + ((long long)b * p.T * p.Hkv + kvh) * D);
+    const char* vn = reinterpret_cast<const char*>(Vn + ((long long)b * p.T * p.Hkv + kvh) * D);
+
+    // Block blk of this wave's ring into a stage: each of the NR row waves brings its share
+    // of the 1 KB pieces of K and V.
+    auto issue = [&](int stage, int blk) __attribute__((always_inline)) {
+      const bool tail = blk >= ncb;
+      const int k0 = (tail ? blk - ncb : blk) * 32;
+      const int n = min(32, (tail ? p.T : Lc) - k0);
+      const int ld = tail ? p.Hkv * D : D;                  // elements between rows
+      const long long off = (long long)k0 * ld * 2;
+      const unsigned len = (unsigned)((n - 1) * ld + D) * 2u;
+      const Rsrc rk = make_rsrc((tail ? kn : kc) + off, len), rv = make_rsrc((tail ? vn : vc) + off, len);
+      const unsigned m0 = lds_u32(ring + stage * 2 * TILE);
+#pragma unroll
+      for (int j = 0; j < C::IPW; ++j) {
+        const int i = j * NR + rw;                          // piece: K's, then V's
+        if (2 * C::LD < NR && i >= 2 * C::LD) break;
+        const int slot = (i % C::LD) * 64 + lane, row = slot / C::CH;
+        const unsigned voff = (unsigned)(row * ld + ((slot % C::CH) ^ swz<D>(row)) * 8) * 2u;
+        if (i < C::LD) dma16_buf(rk, voff, m0 + (unsigned)(1024 * i));
+        else dma16_buf(rv, voff, m0 + (unsigned)(1024 * i));
+      }
+    };
+    const int steps = (blk1 - blk0 + NK - 1) / NK;
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+      if (blk0 + s * NK + kw < blk1) issue(s, blk0 + s * NK + kw);
+
+    // The wave's rows, in flight with the first blocks.
+    const int r = (grp * NR + rw) * 32 + l32;
+    const bool row = r < p.R;
+    const int t = row ? r / p.rep : 0;
+    frag qf[DS];
+    const T* qrow = Q + (((long long)b * p.T + t) * p.H + kvh * p.rep + (row ? r % p.rep : 0)) * D;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = row ? ld_frag<T>(qrow + ds * 16 + g * 8) : zero_frag<T>();
+    WaveTree wt = {0u, 0u, -1};
+    bool dead = false, poisoned = false;
+    if (TREE && has_tail) {
+      if (small_tree) {
+        wt = wave_tree(p, b);
+        wt = {__shfl(wt.lo, t), __shfl(wt.hi, t), __shfl(wt.up, t)};
+        dead = wt.up != -1;
+      } else {
+        tree_build(tree, p, b);
+        dead = tree.up[t] != -1;
+      }
+    }
+    f32x16 o[MAPS][DT];
+    float m[MAPS], l[MAPS];
+#pragma unroll
+    for (int x = 0; x < MAPS; ++x) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[x][dt] = zero16();
+      m[x] = kStepNegInit;
+      l[x] = 0.f;
+    }
+    // Retires the Q loads where the compiler sees it (else it drains the ring in the loop).
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+
+    int stage = 0;
+    for (int s = 0; s < steps; ++s) {
+      const int blk = blk0 + s * NK + kw;
+      // This stage has landed; at most NS - 2 later ones are still on their way.
+      if constexpr (NS == 2) {
+        wait_vm<0>();
+      } else {
+        if (blk + (NS - 2) * NK < blk1) wait_vm<(NS - 2) * C::IPW>();
+        else wait_vm<0>();
+      }
+      if constexpr (NR > 1) lds_barrier();   // everybody's pieces, and the slot refilled now is read
+      const int fill = stage == 0 ? NS - 1 : stage - 1;
+      if (blk + (NS - 1) * NK < blk1) issue(fill, blk + (NS - 1) * NK);
+      const char* sK = ring + stage * 2 * TILE;
+      const char* sV = sK + TILE;
+      stage = stage + 1 == NS ? 0 : stage + 1;
+
+      const bool tail = blk >= ncb && blk < blk1;
+      if (TREE && (NR > 1 ? has_tail && blk0 + s * NK + NK > ncb : tail)) {
+        // A value that is not finite would reach every row of the product (0 * inf): its
+        // key is taken out of the tile, and the rows that see it are NaN as a whole.
+        unsigned badw = 0u;
+        if (tail) {
+          constexpr unsigned e = std::is_same_v<T, __bf16> ? 0x7f80u : 0x7c00u;
+          for (int i = lane; i < 32 * C::CH; i += 64) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(sV + 16 * i);
+            bool nf = false;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) nf |= (x[w] & e) == e || ((x[w] >> 16) & e) == e;
+            // Lanes of a row are neighbours: CH of them.
+            const unsigned long long any = __builtin_amdgcn_ballot_w64(nf);
+#pragma unroll
+            for (int q = 0; q < 64 / C::CH; ++q)
+              if ((any >> (q * C::CH)) & ((1ull << (C::CH - 1)) * 2ull - 1ull))
+                badw |= 1u << (i / 64 * (64 / C::CH) + q);
+          }
+        }
+        if constexpr (NR > 1) lds_barrier();   // all have looked before any of them writes
+        if (badw) {
+          for (int i = lane; i < 32 * C::CH; i += 64)
+            if ((badw >> (i / C::CH)) & 1u)
+              *reinterpret_cast<u32x4*>(const_cast<char*>(sV) + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+          const unsigned w = small_tree ? (blk - ncb ? wt.hi : wt.lo) : tree.line[t][blk - ncb];
+          poisoned |= !dead && (w & badw) != 0u;
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+      }
+      if (blk >= blk1) continue;
+
+      f32x16 sc[MAPS];
+#pragma unroll
+      for (int x = 0; x < MAPS; ++x) {
+        sc[x] = zero16();
+#pragma unroll
+        for (int ds = x * DM; ds < (x + 1) * DM; ++ds) sc[x] = M::mma(lds_frag<T>(sK + kaddr[ds]), qf[ds], sc[x]);
+      }
+      if (tail || blk * 32 + 32 > Lc) {
+        unsigned see;
+        if (!tail) see = (1u << (Lc - blk * 32)) - 1u;      // 1 .. 31 rows
+        else if (!TREE) see = chain_word(p, t, blk - ncb);
+        else see = dead ? 0u : small_tree ? (blk - ncb ? wt.hi : wt.lo) : tree.line[t][blk - ncb];
+#pragma unroll
+        for (int x = 0; x < MAPS; ++x) mask_keep(sc[x], see >> (4 * g), -INFINITY);
+      }
+#pragma unroll
+      for (int x = 0; x < MAPS; ++x) {
+        float mx = sc[x][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, sc[x][i]);
+        // The running max moves only when it grows by more than 8 in log2 units.
+        if (wave_any(mx > m[x] + p.resc_th)) {
+          const float m_new = fmaxf(m[x], halves_max(mx));
+          const float alpha = fast_exp2((m[x] - m_new) * c);
+          l[x] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[x][dt][i] *= alpha;
+          m[x] = m_new;
+        }
+        const float mc = m[x] * c;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[x][i] = fast_exp2(fmaf(sc[x][i], c, -mc));
+          rs[i & 3] += sc[x][i];
+        }
+        l[x] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        frag pf[MAPS];
+#pragma unroll
+        for (int x = 0; x < MAPS; ++x) pf[x] = pack_frag<T>(sc[x], ks * 8);
+        const int roff = 16 * ks * D * 2;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const frag vt = lds_frag_tr<T>(sV + vaddr[dt][0] + roff, sV + vaddr[dt][1] + roff);
+#pragma unroll
+          for (int x = 0; x < MAPS; ++x) o[x][dt] = M::mma(vt, pf[x], o[x][dt]);
+        }
+      }
+    }
+
+    // The fragment's result. l < 0 marks a row outside the tree, m = NaN a poisoned one.
+    const int slot = 2 * blockIdx.x + (at != (long long)blockIdx.x * line.per);
+    float* po = part + (long long)slot * C::SLOT;
+    float* pml = po + C::ROWS * MAPS * D;
+#pragma unroll
+    for (int x = 0; x < MAPS; ++x) {
+      l[x] = halves_sum(l[x]);
+      if (dead) l[x] = -1.f;
+      if (poisoned) m[x] = NAN;
+    }
+    if constexpr (NK == 1) {
+      if (row) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int d0 = dt * 32 + 8 * j + 4 * g;
+            f32x4 v[MAPS];
+#pragma unroll
+            for (int x = 0; x < MAPS; ++x)
+              v[x] = f32x4{o[x][dt][4 * j], o[x][dt][4 * j + 1], o[x][dt][4 * j + 2], o[x][dt][4 * j + 3]};
+            if (whole) {
+              step16_emit<T, D, MAPS>(p, O, LSE, b, kvh, r, d0, v, m, l, dead, poisoned);
+            } else {
+#pragma unroll
+              for (int x = 0; x < MAPS; ++x)
+                *reinterpret_cast<f32x4*>(po + ((rw * 32 + l32) * MAPS + x) * D + d0) = v[x];
+            }
+          }
+        if (!whole && g == 0) {
+#pragma unroll
+          for (int x = 0; x < MAPS; ++x) {
+            pml[(rw * 32 + l32) * 2 * MAPS + 2 * x] = m[x];
+            pml[(rw * 32 + l32) * 2 * MAPS + 2 * x + 1] = l[x];
+          }
+        }
+      }
+      __syncthreads();   // the ring is free for the next fragment
+    } else {
+      __syncthreads();   // every wave has left the ring
+      // Quad q of a row at q ^ row: the rows' quads in different banks.
+      float* ob = reinterpret_cast<float*>(lds);
+      constexpr int NQ = D / 4;
+#pragma unroll
+      for (int x = 0; x < MAPS; ++x) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 v = {o[x][dt][4 * j], o[x][dt][4 * j + 1], o[x][dt][4 * j + 2], o[x][dt][4 * j + 3]};
+            const int q = (dt * 8 + 2 * j + g) ^ (l32 & (NQ - 1));
+            *reinterpret_cast<f32x4*>(ob + ((wave * 32 + l32) * MAPS + x) * D + 4 * q) = v;
+          }
+        if (g == 0) {
+          ml[wave][l32][2 * x] = m[x];
+          ml[wave][l32][2 * x + 1] = l[x];
+        }
+      }
+      __syncthreads();
+      const int rows = min(p.R - grp * C::ROWS, C::ROWS);
+      for (int i = tid; i < rows * NQ; i += NT) {
+        const int rr = i / NQ, q = i % NQ, w0 = rr >> 5, rl = rr & 31;
+        f32x4 v[MAPS];
+        float Mx[MAPS], L[MAPS];
+        bool gone = false, nan = false;
+#pragma unroll
+        for (int x = 0; x < MAPS; ++x) {
+          Mx[x] = ml[w0][rl][2 * x];
+#pragma unroll
+          for (int k = 1; k < NK; ++k) Mx[x] = fmaxf(Mx[x], ml[k * NR + w0][rl][2 * x]);
+          v[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+          L[x] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            const float mk = ml[k * NR + w0][rl][2 * x], lk = ml[k * NR + w0][rl][2 * x + 1];
+            gone |= lk < 0.f;
+            nan |= mk != mk;
+            const float a = fast_exp2((mk - Mx[x]) * c);
+            L[x] += a * lk;
+            v[x] += a * *reinterpret_cast<const f32x4*>(
+                            ob + (((k * NR + w0) * 32 + rl) * MAPS + x) * D + 4 * (q ^ (rl & (NQ - 1))));
+          }
+        }
+        if (whole) {
+          step16_emit<T, D, MAPS>(p, O, LSE, b, kvh, grp * C::ROWS + rr, 4 * q, v, Mx, L, gone, nan);
+        } else {
+#pragma unroll
+          for (int x = 0; x < MAPS; ++x) {
+            *reinterpret_cast<f32x4*>(po + (rr * MAPS + x) * D + 4 * q) = v[x];
+            if (q == 0) {
+              pml[rr * 2 * MAPS + 2 * x] = nan ? NAN : Mx[x];
+              pml[rr * 2 * MAPS + 2 * x + 1] = gone ? -1.f : L[x];
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    at += blk1 - blk0;
+    if (at >= end) break;
+    if (at == (before + nb) * ups) {       // the sequence's last unit is done
+      before += nb;
+      ++b;
+    }
+  }
+}
+
+// The units that several workgroups share, merged in order: a wave per query row.
+template <typename T, int D, int MAPS, int NR, int NK>
+__global__ void __launch_bounds__(256)
+step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* __restrict__ LSE,
+                      StepParams p) {
+  using C = Step16<D, MAPS, NR, NK>;
+  constexpr int NQ = D / 4, FG = 64 / NQ;          // lanes per row, fragments read at once
+  const long long gr = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);   // (b, kvh, r)
+  if (gr >= (long long)p.B * p.Hkv * p.R) return;                        // whole waves
+  const int r = (int)(gr % p.R), kvh = (int)(gr / p.R % p.Hkv), b = (int)(gr / p.R / p.Hkv);
+  const int lane = threadIdx.x & 63, q = lane % NQ, fg = lane / NQ;
+  const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;
+  const Line line = step_line(p, ups);
+  const int nb = step_blocks(p, b), grp = r / C::ROWS, rr = r % C::ROWS;
+  const long long first = blocks_before(p, b) * ups + (long long)(kvh * ngrp + grp) * nb, last = first + nb - 1;
+  const long long g0 = first / line.per, g1 = last / line.per;
+  if (g0 == g1) return;                            // written by the workgroup that had it all
+  const float c = p.scale_log2;
+  f32x4 o[MAPS];
+  float M[MAPS], L[MAPS];
+  bool dead = false, poisoned = false;
+#pragma unroll
+  for (int x = 0; x < MAPS; ++x) {
+    o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    M[x] = kStepNegInit;
+    L[x] = 0.f;
+  }
+  for (long long w = g0 + fg; w <= g1; w += FG) {
+    const float* po = part + (2 * w + (w == g0 && first != g0 * line.per)) * C::SLOT;
+    const float* pml = po + C::ROWS * MAPS * D + rr * 2 * MAPS;
+#pragma unroll
+    for (int x = 0; x < MAPS; ++x) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(po + (rr * MAPS + x) * D + 4 * q);
+      const float mk = pml[2 * x], lk = pml[2 * x + 1];
+      dead |= lk < 0.f;
+      poisoned |= mk != mk;
+      const float mn = fmaxf(M[x], mk);
+      const float a = fast_exp2((M[x] - mn) * c), f = fast_exp2((mk - mn) * c);
+      L[x] = L[x] * a + lk * f;
+      o[x] = o[x] * a + v * f;
+      M[x] = mn;
+    }
+  }
+#pragma unroll
+  for (int off = NQ; off < 64; off <<= 1) {
+    dead |= __shfl_xor((int)dead, off) != 0;
+    poisoned |= __shfl_xor((int)poisoned, off) != 0;
+#pragma unroll
+    for (int x = 0; x < MAPS; ++x) {
+      const float mo = __shfl_xor(M[x], off), lo = __shfl_xor(L[x], off);
+      f32x4 oo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oo[e] = __shfl_xor(o[x][e], off);
+      const float mn = fmaxf(M[x], mo);
+      const float a = fast_exp2((M[x] - mn) * c), f = fast_exp2((mo - mn) * c);
+      L[x] = L[x] * a + lo * f;
+      o[x] = o[x] * a + oo * f;
+      M[x] = mn;
+    }
+  }
+  if (fg == 0) step16_emit<T, D, MAPS>(p, O, LSE, b, kvh, r, 4 * q, o, M, L, dead, poisoned);
+}
+
+namespace {
+
+// Workgroups of a launch: what the chip holds at once (by LDS and registers), fewer where
+// the longest batch that the cache can hold has less than min_blocks for each.
+template <int D, int MAPS, int NR, int NK>
+void step16_geometry(StepParams& p) {
+  using C = Step16<D, MAPS, NR, NK>;
+  constexpr int per_cu = C::LDS > 80 * 1024 ? 1 : C::W == 8 || MAPS * D > 128 || C::LDS > 40 * 1024 ? 2 : 4;
+  const int ngrp = (p.R + C::ROWS - 1) / C::ROWS;
+  const long long most = (long long)p.B * p.Hkv * ngrp * ((p.rows + 31) / 32 + (p.T + 31) / 32);
+  p.min_blocks = 4 * NK;
+  const long long want = (most + p.min_blocks - 1) / p.min_blocks;
+  p.nsplit = (int)(want < 256 * per_cu ? want : 256 * per_cu);
+}
+
+template <typename T, int D, int MAPS, int NR, int NK>
+hipError_t step16_t(const void* q, const void* kc, const void* vc, const void* kn, const void* vn, void* out,
+                    float* lse, float* ws, StepParams p, hipStream_t st) {
+  step16_geometry<D, MAPS, NR, NK>(p);
+  const auto go = [&](auto tree) {
+    hipLaunchKernelGGL((step16_kernel<T, D, MAPS, NR, NK, decltype(tree)::value>), dim3((unsigned)p.nsplit),
+                       dim3(64 * NR * NK), 0, st, (const T*)q, (const T*)kc, (const T*)vc, (const T*)kn,
+                       (const T*)vn, (T*)out, lse, ws, p);
+  };
+  if (p.parents) go(std::true_type{});
+  else go(std::false_type{});
+  const long long rows = (long long)p.B * p.Hkv * p.R;
+  hipLaunchKernelGGL((step16_combine_kernel<T, D, MAPS, NR, NK>), dim3((unsigned)((rows + 3) / 4)), dim3(256),
+                     0, st, ws, (T*)out, lse, p);
+  return hipGetLastError();
+}
+
+template <int I>
+using ic = std::integral_constant<int, I>;
+
+// f(D, MAPS, NR, NK) for a step: row waves by the row tiles of a kv head.
+template <typename F>
+auto step16_by_shape(const StepParams& p, int D, bool two_maps, F f) {
+  const auto by_rows = [&](auto d, auto maps) {
+    const int tiles = (p.R + 31) / 32;
+    if (tiles <= 1) return f(d, maps, ic<1>{}, ic<4>{});
+    if (tiles <= 2) return f(d, maps, ic<2>{}, ic<2>{});
+    // (Eight waves of two 128-wide maps do not fit the registers.)
+    if constexpr (decltype(d)::value * decltype(maps)::value <= 128) {
+      if (tiles > 4) return f(d, maps, ic<8>{}, ic<1>{});
+    }
+    return f(d, maps, ic<4>{}, ic<1>{});
+  };
+  const auto by_maps = [&](auto d) { return two_maps ? by_rows(d, ic<2>{}) : by_rows(d, ic<1>{}); };
+  return D == 32 ? by_maps(ic<32>{}) : D == 64 ? by_maps(ic<64>{}) : by_maps(ic<128>{});
+}
+
+}  // namespace
+
+long long step16_workspace_floats(const StepParams& p, int D, bool two_maps) {
+  return step16_by_shape(p, D, two_maps, [&](auto d, auto m, auto nr, auto nk) {
+    using C = Step16<decltype(d)::value, decltype(m)::value, decltype(nr)::value, decltype(nk)::value>;
+    StepParams g = p;
+    step16_geometry<decltype(d)::value, decltype(m)::value, decltype(nr)::value, decltype(nk)::value>(g);
+    return 2LL * g.nsplit * C::SLOT;
+  });
+}
+
+hipError_t launch_step16(int dtype, int D, const void* q, const void* kc, const void* vc, const void* kn,
+                         const void* vn, void* out, float* lse, float* ws, const StepParams& p,
+                         hipStream_t st) {
+  return step16_by_shape(p, D, p.lam != nullptr, [&](auto d, auto m, auto nr, auto nk) {
+    constexpr int DD = decltype(d)::value, MM = decltype(m)::value, RR = decltype(nr)::value,
+                  KK = decltype(nk)::value;
+    return dtype == 1 ? step16_t<_Float16, DD, MM, RR, KK>(q, kc, vc, kn, vn, out, lse, ws, p, st)
+                      : step16_t<__bf16, DD, MM, RR, KK>(q, kc, vc, kn, vn, out, lse, ws, p, st);
+  });
+}
+
+}  // namespace mi

@@ -884,8 +884,11 @@ int validate_step(const mi_step_shape* s) {
                              s->k_batch_stride, s->k_head_stride, s->v_batch_stride, s->v_head_stride};
   const int st = validate_dec(&d);
   if (st) return st;
-  // Query rows of a kv head and rows of the step are 32-bit in the kernels.
+  // The step's query rows, and the bytes of 32 rows of the active block, are 32-bit in the
+  // kernels.
   if ((long long)s->B * s->T * s->H > 0x7fffffffLL) return MI_ERR_SIZE;
+  if (32LL * s->Hkv * s->D * 4 > 0x7fffffffLL) return MI_ERR_SIZE;
+  if ((long long)s->rows + s->T > 0x7fffff00LL) return MI_ERR_SIZE;
   return MI_OK;
 }
 
@@ -907,6 +910,7 @@ mi::StepParams step_params(const mi_step_shape* s) {
   p.parents_sb = s->one_tree ? 0 : s->T;
   p.lam_dtype = s->lam_dtype;
   p.R = s->T * p.rep;
+  p.resc_th = 8.f / p.scale_log2;
   return p;
 }
 
