@@ -2,16 +2,19 @@
 // the whole batch dealt evenly to the workgroups.
 //
 //  * Work. A unit is one (sequence, kv head, group of NR row tiles of 32 query rows); its
-//    key blocks, unit after unit, form one line of N blocks, cut into equal pieces, one per
-//    workgroup: sequences of any lengths load the chip evenly. (Cut per sequence, the
-//    longest one sets the time.) The lengths are on the GPU, so each workgroup finds its
-//    piece itself, from a prefix sum over them. A piece is one or more fragments of units;
+//    key blocks, unit after unit, form one line, cut into equal pieces, one per workgroup:
+//    sequences of any lengths load the chip evenly. (Cut per sequence, the longest one sets
+//    the time.) Each unit has SETUP empty blocks in front: a piece that reaches into
+//    another unit starts its loads anew and writes twice, so it gets fewer keys. The
+//    lengths are on the GPU, so each workgroup finds its piece itself, from a prefix sum
+//    over them. A piece is one or more fragments of units;
 //    a unit that one fragment covers is written at once, the others' fragments go to the
 //    workspace as float32 partials (at most the first and the last of a piece are partial:
 //    two slots per workgroup) and step16_combine_kernel merges them in order.
-//  * Waves. NR row waves x NK key waves: up to 32 rows, each of four waves takes every
-//    fourth block (its own LDS ring, no barrier in the loop); with more rows, waves share
-//    the blocks of a ring. A wave's scores are transposed, S^T = K Q^T, so a lane owns a
+//  * Waves. NR row waves x NM map waves x NK key groups. Up to 32 rows, each of four waves
+//    takes every fourth block (its own LDS ring, no barrier in the loop) and both maps;
+//    with more rows, a group's waves share the blocks of its ring, a row tile and a map
+//    each (two 128-wide maps' sums of 32 rows would fill half of the registers). A wave's scores are transposed, S^T = K Q^T, so a lane owns a
 //    query row and P^T feeds O^T += V^T P^T from registers (attn16.h's tiles).
 //  * Masks only where a block needs one: a sequence's last cached block (rows past it read
 //    as zeros through the buffer's bound) and the active block's, one word per block.
@@ -27,63 +30,67 @@ namespace {
 
 template <int D, int MAPS, int NR, int NK>
 struct Step16 {
-  static constexpr int W = NR * NK;              // waves
+  static constexpr int MW = NR == 1 ? MAPS : 1;  // maps of a wave
+  static constexpr int NM = MAPS / MW, NG = NR * NM;   // map waves; waves that share a ring
+  static constexpr int W = NG * NK;              // waves
   static constexpr int CH = D / 8;               // 16-byte chunks per row
   static constexpr int TILE = 32 * D * 2;        // K (or V) of a block
   static constexpr int LD = TILE / 1024;         // DMA instructions per tile
-  static constexpr int IPW = 2 * LD >= NR ? 2 * LD / NR : 1;   // ... of K and V per wave
+  static constexpr int IPW = 2 * LD >= NG ? 2 * LD / NG : 1;   // ... of K and V per wave
   static constexpr int NS = NK == 4 ? 2 : 3;     // ring stages
+  static constexpr int SETUP = 16;               // what starting a unit costs, in blocks
   static constexpr int RING = NK * NS * 2 * TILE;
-  // Key waves' float32 results, merged in LDS (the ring's bytes, after the loop).
-  static constexpr int MERGE = NK > 1 ? W * 32 * MAPS * D * 4 : 0;
+  // The waves' float32 results, merged in LDS (the ring's bytes, after the loop).
+  static constexpr bool JOIN = NK * NM > 1;
+  static constexpr int MERGE = JOIN ? W * 32 * MW * D * 4 : 0;
   static constexpr int LDS = RING > MERGE ? RING : MERGE;
-  static constexpr int DS = D / 16, DM = DS / MAPS, DT = D / 32;
+  static constexpr int DS = D / 16 / NM, DM = DS / MW, DT = D / 32;   // k-steps: a wave's, a map's
   // A slot: the rows' O of each map, then their (m, l).
   static constexpr int ROWS = NR * 32, SLOT = ROWS * (MAPS * D + 2 * MAPS);
 };
 
-// The line of blocks: N of them, `per` to a workgroup.
+// The line of blocks: N of them, `per` to a workgroup (N fits 31 bits: validated).
 struct Line {
-  long long N, per;
+  int N, per;
 };
 
-// A value that is the same in every lane, in scalar registers.
+// A value that is the same in every lane, in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uniform(long long x) {
-  const unsigned lo = (unsigned)uniform((int)x), hi = (unsigned)uniform((int)(x >> 32));
-  return (long long)((unsigned long long)hi << 32 | lo);
-}
 
+// Blocks of a unit of sequence b, the empty ones included.
+template <int SETUP>
 __device__ __forceinline__ int step_blocks(const StepParams& p, int b) {
-  return (step_len(p, b) + 31) / 32 + (p.T + 31) / 32;
+  return (step_len(p, b) + 31) / 32 + (p.T + 31) / 32 + SETUP;
 }
 
-// Blocks of the sequences before `b` (each counted once), all lanes of a wave.
-__device__ __forceinline__ long long blocks_before(const StepParams& p, int b) {
-  long long sum = 0;
-  for (int i = threadIdx.x & 63; i < b; i += 64) sum += step_blocks(p, i);
+// Blocks of one unit of each sequence before `b`, all lanes of a wave.
+template <int SETUP>
+__device__ __forceinline__ int blocks_before(const StepParams& p, int b) {
+  int sum = 0;
+  for (int i = threadIdx.x & 63; i < b; i += 64) sum += step_blocks<SETUP>(p, i);
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
   return uniform(sum);
 }
 
+template <int SETUP>
 __device__ __forceinline__ Line step_line(const StepParams& p, int units_per_seq) {
-  const long long N = blocks_before(p, p.B) * units_per_seq;
-  const long long per = (N + p.nsplit - 1) / p.nsplit;
-  return {N, per > p.min_blocks ? per : p.min_blocks};
+  const int N = blocks_before<SETUP>(p, p.B) * units_per_seq;
+  return {N, max((int)(((unsigned)N + p.nsplit - 1) / (unsigned)p.nsplit), p.min_blocks)};
 }
 
-// The sequence that holds block x (x < N / units) of the sequences' blocks counted once,
-// and the blocks before it: a wave's scan, 64 sequences a round.
-__device__ __forceinline__ int find_seq(const StepParams& p, long long x, long long& before) {
+// The sequence that holds block x of one unit of each sequence, and the blocks before it:
+// a wave's scan, 64 sequences a round.
+template <int SETUP>
+__device__ __forceinline__ int find_seq(const StepParams& p, int x, int& before) {
   const int lane = threadIdx.x & 63;
   before = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int own = b0 + lane < p.B ? step_blocks(p, b0 + lane) : 0;
-    long long upto = own;
+    const int own = b0 + lane < p.B ? step_blocks<SETUP>(p, b0 + lane) : 0;
+    int upto = own;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-      const long long y = __shfl_up(upto, s);
+      const int y = __shfl_up(upto, s);
       if (lane >= s) upto += y;
     }
     const unsigned long long past = __builtin_amdgcn_ballot_w64(before + upto > x);
@@ -142,7 +149,7 @@ __device__ __forceinline__ void step16_emit(const StepParams& p, T* __restrict__
 }  // namespace
 
 template <typename T, int D, int MAPS, int NR, int NK, bool TREE>
-__global__ void __launch_bounds__(64 * NR * NK)
+__global__ void __launch_bounds__((64 * Step16<D, MAPS, NR, NK>::W))
 step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __restrict__ Vc,
               const T* __restrict__ Kn, const T* __restrict__ Vn, T* __restrict__ O,
               float* __restrict__ LSE, float* __restrict__ part, StepParams p) {
@@ -150,25 +157,29 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   using M = Mfma32<T>;
   using frag = typename M::frag;
   constexpr int NS = C::NS, DS = C::DS, DM = C::DM, DT = C::DT, TILE = C::TILE, NT = 64 * C::W;
+  constexpr int MW = C::MW, NM = C::NM, NG = C::NG;
   static_assert(NT >= kTreeMax, "tree_build wants a thread per node");
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
-  __shared__ float ml[NK > 1 ? C::W : 1][32][2 * MAPS];
+  __shared__ float ml[C::JOIN ? C::W : 1][32][2 * MW];
   __shared__ TreeLds tree;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, g = lane >> 5;
-  const int rw = wave % NR, kw = wave / NR;
+  const int rw = wave % NR, mw = wave / NR % NM, kw = wave / NG;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;   // units per sequence
-  const Line line = step_line(p, ups);
-  long long at = (long long)blockIdx.x * line.per;
-  const long long end = at + line.per < line.N ? at + line.per : line.N;
-  if (at >= end) return;
+  const Line line = step_line<C::SETUP>(p, ups);
+  // (Pieces past the line's end: none of the products passes 31 bits, nsplit and per being
+  // chosen for the largest N.)
+  const long long begin = (long long)blockIdx.x * line.per;
+  if (begin >= line.N) return;
+  int at = (int)begin;
+  const int end = line.N - at > line.per ? at + line.per : line.N;
 
   char* ring = lds + kw * (NS * 2 * TILE);
   int kaddr[DS];
 #pragma unroll
-  for (int ds = 0; ds < DS; ++ds) kaddr[ds] = tile_off<D>(l32, 2 * ds + g);
+  for (int ds = 0; ds < DS; ++ds) kaddr[ds] = tile_off<D>(l32, 2 * (mw * DS + ds) + g);
   int vaddr[DT][2];
   {
     const int G = lane >> 4, m = lane & 15, row = 4 * (G >> 1) + (m >> 2);
@@ -182,23 +193,24 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   const float c = p.scale_log2;
   const bool small_tree = TREE && p.T <= 64;
 
-  long long before;                       // blocks of earlier sequences, counted once
-  int b = find_seq(p, at / ups, before);
+  int before;                             // blocks of one unit of each earlier sequence
+  int b = find_seq<C::SETUP>(p, at / ups, before);
   while (true) {
-    // The fragment [at, stop) of unit u of sequence b.
+    // The fragment of unit u of sequence b that begins at `at`: its blocks [blk0, blk1).
     const int Lc = step_len(p, b), ncb = (Lc + 31) / 32, nb = ncb + (p.T + 31) / 32;
-    const long long in_seq = at - before * ups;
-    const int u = (int)(in_seq / nb), blk0 = (int)(in_seq - (long long)u * nb);
-    const int blk1 = (int)min((long long)nb, blk0 + (end - at));
+    const int span = nb + C::SETUP, in_seq = at - before * ups;
+    const int u = in_seq / span, from = in_seq - u * span, to = min(span, from + end - at);
+    const int blk0 = max(from - C::SETUP, 0), blk1 = to - C::SETUP;
     const int kvh = u / ngrp, grp = u % ngrp;
     const bool whole = blk0 == 0 && blk1 == nb, has_tail = blk1 > ncb;
+    if (blk1 > blk0) {
 
     const char* kc = reinterpret_cast<const char*>(Kc + (long long)b * p.k_sb + (long long)kvh * p.k_sh);
     const char* vc = reinterpret_cast<const char*>(Vc + (long long)b * p.v_sb + (long long)kvh * p.v_sh);
     const char* kn = reinterpret_cast<const char*>(Kn + ((long long)b * p.T * p.Hkv + kvh) * D);
     const char* vn = reinterpret_cast<const char*>(Vn + ((long long)b * p.T * p.Hkv + kvh) * D);
 
-    // Block blk of this wave's ring into a stage: each of the NR row waves brings its share
+    // Block blk of this wave's ring into a stage: each of the NG waves brings its share
     // of the 1 KB pieces of K and V.
     auto issue = [&](int stage, int blk) __attribute__((always_inline)) {
       const bool tail = blk >= ncb;
@@ -211,8 +223,8 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       const unsigned m0 = lds_u32(ring + stage * 2 * TILE);
 #pragma unroll
       for (int j = 0; j < C::IPW; ++j) {
-        const int i = j * NR + rw;                          // piece: K's, then V's
-        if (2 * C::LD < NR && i >= 2 * C::LD) break;
+        const int i = j * NG + wave % NG;                   // piece: K's, then V's
+        if (2 * C::LD < NG && i >= 2 * C::LD) break;
         const int slot = (i % C::LD) * 64 + lane, row = slot / C::CH;
         const unsigned voff = (unsigned)(row * ld + ((slot % C::CH) ^ swz<D>(row)) * 8) * 2u;
         if (i < C::LD) dma16_buf(rk, voff, m0 + (unsigned)(1024 * i));
@@ -231,7 +243,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
     frag qf[DS];
     const T* qrow = Q + (((long long)b * p.T + t) * p.H + kvh * p.rep + (row ? r % p.rep : 0)) * D;
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qf[ds] = row ? ld_frag<T>(qrow + ds * 16 + g * 8) : zero_frag<T>();
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = row ? ld_frag<T>(qrow + (mw * DS + ds) * 16 + g * 8) : zero_frag<T>();
     WaveTree wt = {0u, 0u, -1};
     bool dead = false, poisoned = false;
     if (TREE && has_tail) {
@@ -244,10 +256,10 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
         dead = tree.up[t] != -1;
       }
     }
-    f32x16 o[MAPS][DT];
-    float m[MAPS], l[MAPS];
+    f32x16 o[MW][DT];
+    float m[MW], l[MW];
 #pragma unroll
-    for (int x = 0; x < MAPS; ++x) {
+    for (int x = 0; x < MW; ++x) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[x][dt] = zero16();
       m[x] = kStepNegInit;
@@ -266,7 +278,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
         if (blk + (NS - 2) * NK < blk1) wait_vm<(NS - 2) * C::IPW>();
         else wait_vm<0>();
       }
-      if constexpr (NR > 1) lds_barrier();   // everybody's pieces, and the slot refilled now is read
+      if constexpr (NG > 1) lds_barrier();   // everybody's pieces, and the slot refilled now is read
       const int fill = stage == 0 ? NS - 1 : stage - 1;
       if (blk + (NS - 1) * NK < blk1) issue(fill, blk + (NS - 1) * NK);
       const char* sK = ring + stage * 2 * TILE;
@@ -274,7 +286,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       stage = stage + 1 == NS ? 0 : stage + 1;
 
       const bool tail = blk >= ncb && blk < blk1;
-      if (TREE && (NR > 1 ? has_tail && blk0 + s * NK + NK > ncb : tail)) {
+      if (TREE && (NG > 1 ? has_tail && blk0 + s * NK + NK > ncb : tail)) {
         // A value that is not finite would reach every row of the product (0 * inf): its
         // key is taken out of the tile, and the rows that see it are NaN as a whole.
         unsigned badw = 0u;
@@ -293,7 +305,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
                 badw |= 1u << (i / 64 * (64 / C::CH) + q);
           }
         }
-        if constexpr (NR > 1) lds_barrier();   // all have looked before any of them writes
+        if constexpr (NG > 1) lds_barrier();   // all have looked before any of them writes
         if (badw) {
           for (int i = lane; i < 32 * C::CH; i += 64)
             if ((badw >> (i / C::CH)) & 1u)
@@ -305,9 +317,9 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       }
       if (blk >= blk1) continue;
 
-      f32x16 sc[MAPS];
+      f32x16 sc[MW];
 #pragma unroll
-      for (int x = 0; x < MAPS; ++x) {
+      for (int x = 0; x < MW; ++x) {
         sc[x] = zero16();
 #pragma unroll
         for (int ds = x * DM; ds < (x + 1) * DM; ++ds) sc[x] = M::mma(lds_frag<T>(sK + kaddr[ds]), qf[ds], sc[x]);
@@ -318,10 +330,10 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
         else if (!TREE) see = chain_word(p, t, blk - ncb);
         else see = dead ? 0u : small_tree ? (blk - ncb ? wt.hi : wt.lo) : tree.line[t][blk - ncb];
 #pragma unroll
-        for (int x = 0; x < MAPS; ++x) mask_keep(sc[x], see >> (4 * g), -INFINITY);
+        for (int x = 0; x < MW; ++x) mask_keep(sc[x], see >> (4 * g), -INFINITY);
       }
 #pragma unroll
-      for (int x = 0; x < MAPS; ++x) {
+      for (int x = 0; x < MW; ++x) {
         float mx = sc[x][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, sc[x][i]);
@@ -347,54 +359,44 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        frag pf[MAPS];
+        frag pf[MW];
 #pragma unroll
-        for (int x = 0; x < MAPS; ++x) pf[x] = pack_frag<T>(sc[x], ks * 8);
+        for (int x = 0; x < MW; ++x) pf[x] = pack_frag<T>(sc[x], ks * 8);
         const int roff = 16 * ks * D * 2;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const frag vt = lds_frag_tr<T>(sV + vaddr[dt][0] + roff, sV + vaddr[dt][1] + roff);
 #pragma unroll
-          for (int x = 0; x < MAPS; ++x) o[x][dt] = M::mma(vt, pf[x], o[x][dt]);
+          for (int x = 0; x < MW; ++x) o[x][dt] = M::mma(vt, pf[x], o[x][dt]);
         }
       }
     }
 
     // The fragment's result. l < 0 marks a row outside the tree, m = NaN a poisoned one.
-    const int slot = 2 * blockIdx.x + (at != (long long)blockIdx.x * line.per);
+    const int slot = 2 * blockIdx.x + (at != (int)begin);
     float* po = part + (long long)slot * C::SLOT;
     float* pml = po + C::ROWS * MAPS * D;
 #pragma unroll
-    for (int x = 0; x < MAPS; ++x) {
+    for (int x = 0; x < MW; ++x) {
       l[x] = halves_sum(l[x]);
       if (dead) l[x] = -1.f;
       if (poisoned) m[x] = NAN;
     }
-    if constexpr (NK == 1) {
+    if constexpr (!C::JOIN) {                // one map, one key group: from the registers
       if (row) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int d0 = dt * 32 + 8 * j + 4 * g;
-            f32x4 v[MAPS];
-#pragma unroll
-            for (int x = 0; x < MAPS; ++x)
-              v[x] = f32x4{o[x][dt][4 * j], o[x][dt][4 * j + 1], o[x][dt][4 * j + 2], o[x][dt][4 * j + 3]};
-            if (whole) {
-              step16_emit<T, D, MAPS>(p, O, LSE, b, kvh, r, d0, v, m, l, dead, poisoned);
-            } else {
-#pragma unroll
-              for (int x = 0; x < MAPS; ++x)
-                *reinterpret_cast<f32x4*>(po + ((rw * 32 + l32) * MAPS + x) * D + d0) = v[x];
-            }
+            const f32x4 v[1] = {
+                {o[0][dt][4 * j], o[0][dt][4 * j + 1], o[0][dt][4 * j + 2], o[0][dt][4 * j + 3]}};
+            if (whole) step16_emit<T, D, 1>(p, O, LSE, b, kvh, r, d0, v, m, l, dead, poisoned);
+            else *reinterpret_cast<f32x4*>(po + (rw * 32 + l32) * D + d0) = v[0];
           }
         if (!whole && g == 0) {
-#pragma unroll
-          for (int x = 0; x < MAPS; ++x) {
-            pml[(rw * 32 + l32) * 2 * MAPS + 2 * x] = m[x];
-            pml[(rw * 32 + l32) * 2 * MAPS + 2 * x + 1] = l[x];
-          }
+          pml[(rw * 32 + l32) * 2] = m[0];
+          pml[(rw * 32 + l32) * 2 + 1] = l[0];
         }
       }
       __syncthreads();   // the ring is free for the next fragment
@@ -404,14 +406,14 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       float* ob = reinterpret_cast<float*>(lds);
       constexpr int NQ = D / 4;
 #pragma unroll
-      for (int x = 0; x < MAPS; ++x) {
+      for (int x = 0; x < MW; ++x) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const f32x4 v = {o[x][dt][4 * j], o[x][dt][4 * j + 1], o[x][dt][4 * j + 2], o[x][dt][4 * j + 3]};
             const int q = (dt * 8 + 2 * j + g) ^ (l32 & (NQ - 1));
-            *reinterpret_cast<f32x4*>(ob + ((wave * 32 + l32) * MAPS + x) * D + 4 * q) = v;
+            *reinterpret_cast<f32x4*>(ob + ((wave * 32 + l32) * MW + x) * D + 4 * q) = v;
           }
         if (g == 0) {
           ml[wave][l32][2 * x] = m[x];
@@ -427,20 +429,22 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
         bool gone = false, nan = false;
 #pragma unroll
         for (int x = 0; x < MAPS; ++x) {
-          Mx[x] = ml[w0][rl][2 * x];
+          // Map x of key group k: wave w0 + x / MW * NR + k * NG.
+          const int w = w0 + x / MW * NR, y = x % MW;
+          Mx[x] = ml[w][rl][2 * y];
 #pragma unroll
-          for (int k = 1; k < NK; ++k) Mx[x] = fmaxf(Mx[x], ml[k * NR + w0][rl][2 * x]);
+          for (int k = 1; k < NK; ++k) Mx[x] = fmaxf(Mx[x], ml[k * NG + w][rl][2 * y]);
           v[x] = f32x4{0.f, 0.f, 0.f, 0.f};
           L[x] = 0.f;
 #pragma unroll
           for (int k = 0; k < NK; ++k) {
-            const float mk = ml[k * NR + w0][rl][2 * x], lk = ml[k * NR + w0][rl][2 * x + 1];
+            const float mk = ml[k * NG + w][rl][2 * y], lk = ml[k * NG + w][rl][2 * y + 1];
             gone |= lk < 0.f;
             nan |= mk != mk;
             const float a = fast_exp2((mk - Mx[x]) * c);
             L[x] += a * lk;
             v[x] += a * *reinterpret_cast<const f32x4*>(
-                            ob + (((k * NR + w0) * 32 + rl) * MAPS + x) * D + 4 * (q ^ (rl & (NQ - 1))));
+                            ob + (((k * NG + w) * 32 + rl) * MW + y) * D + 4 * (q ^ (rl & (NQ - 1))));
           }
         }
         if (whole) {
@@ -458,11 +462,12 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
       }
       __syncthreads();
     }
+    }   // blk1 > blk0
 
-    at += blk1 - blk0;
+    at += to - from;
     if (at >= end) break;
-    if (at == (before + nb) * ups) {       // the sequence's last unit is done
-      before += nb;
+    if (u + 1 == ups) {                    // the sequence's last unit is done
+      before += span;
       ++b;
     }
   }
@@ -480,10 +485,10 @@ step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* 
   const int r = (int)(gr % p.R), kvh = (int)(gr / p.R % p.Hkv), b = (int)(gr / p.R / p.Hkv);
   const int lane = threadIdx.x & 63, q = lane % NQ, fg = lane / NQ;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;
-  const Line line = step_line(p, ups);
-  const int nb = step_blocks(p, b), grp = r / C::ROWS, rr = r % C::ROWS;
-  const long long first = blocks_before(p, b) * ups + (long long)(kvh * ngrp + grp) * nb, last = first + nb - 1;
-  const long long g0 = first / line.per, g1 = last / line.per;
+  const Line line = step_line<C::SETUP>(p, ups);
+  const int span = step_blocks<C::SETUP>(p, b), grp = r / C::ROWS, rr = r % C::ROWS;
+  const int start = blocks_before<C::SETUP>(p, b) * ups + (kvh * ngrp + grp) * span;
+  const int g0 = (start + C::SETUP) / line.per, g1 = (start + span - 1) / line.per;
   if (g0 == g1) return;                            // written by the workgroup that had it all
   const float c = p.scale_log2;
   f32x4 o[MAPS];
@@ -495,8 +500,9 @@ step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* 
     M[x] = kStepNegInit;
     L[x] = 0.f;
   }
-  for (long long w = g0 + fg; w <= g1; w += FG) {
-    const float* po = part + (2 * w + (w == g0 && first != g0 * line.per)) * C::SLOT;
+  for (int w = g0 + fg; w <= g1; w += FG) {
+    // The first of them may have begun with another unit.
+    const float* po = part + (2LL * w + (start > w * line.per)) * C::SLOT;
     const float* pml = po + C::ROWS * MAPS * D + rr * 2 * MAPS;
 #pragma unroll
     for (int x = 0; x < MAPS; ++x) {
@@ -538,9 +544,9 @@ namespace {
 template <int D, int MAPS, int NR, int NK>
 void step16_geometry(StepParams& p) {
   using C = Step16<D, MAPS, NR, NK>;
-  constexpr int per_cu = C::LDS > 80 * 1024 ? 1 : C::W == 8 || MAPS * D > 128 || C::LDS > 40 * 1024 ? 2 : 4;
+  constexpr int per_cu = C::LDS > 80 * 1024 || C::W == 8 ? 1 : 2;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS;
-  const long long most = (long long)p.B * p.Hkv * ngrp * ((p.rows + 31) / 32 + (p.T + 31) / 32);
+  const long long most = (long long)p.B * p.Hkv * ngrp * ((p.rows + 31) / 32 + (p.T + 31) / 32 + C::SETUP);
   p.min_blocks = 4 * NK;
   const long long want = (most + p.min_blocks - 1) / p.min_blocks;
   p.nsplit = (int)(want < 256 * per_cu ? want : 256 * per_cu);
@@ -552,7 +558,7 @@ hipError_t step16_t(const void* q, const void* kc, const void* vc, const void* k
   step16_geometry<D, MAPS, NR, NK>(p);
   const auto go = [&](auto tree) {
     hipLaunchKernelGGL((step16_kernel<T, D, MAPS, NR, NK, decltype(tree)::value>), dim3((unsigned)p.nsplit),
-                       dim3(64 * NR * NK), 0, st, (const T*)q, (const T*)kc, (const T*)vc, (const T*)kn,
+                       dim3(64 * Step16<D, MAPS, NR, NK>::W), 0, st, (const T*)q, (const T*)kc, (const T*)vc, (const T*)kn,
                        (const T*)vn, (T*)out, lse, ws, p);
   };
   if (p.parents) go(std::true_type{});
@@ -573,11 +579,10 @@ auto step16_by_shape(const StepParams& p, int D, bool two_maps, F f) {
     const int tiles = (p.R + 31) / 32;
     if (tiles <= 1) return f(d, maps, ic<1>{}, ic<4>{});
     if (tiles <= 2) return f(d, maps, ic<2>{}, ic<2>{});
-    // (Eight waves of two 128-wide maps do not fit the registers.)
-    if constexpr (decltype(d)::value * decltype(maps)::value <= 128) {
-      if (tiles > 4) return f(d, maps, ic<8>{}, ic<1>{});
-    }
-    return f(d, maps, ic<4>{}, ic<1>{});
+    if constexpr (decltype(maps)::value == 1)
+      return tiles <= 4 ? f(d, maps, ic<4>{}, ic<2>{}) : f(d, maps, ic<8>{}, ic<1>{});
+    else
+      return f(d, maps, ic<4>{}, ic<1>{});
   };
   const auto by_maps = [&](auto d) { return two_maps ? by_rows(d, ic<2>{}) : by_rows(d, ic<1>{}); };
   return D == 32 ? by_maps(ic<32>{}) : D == 64 ? by_maps(ic<64>{}) : by_maps(ic<128>{});

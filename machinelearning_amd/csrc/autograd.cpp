@@ -1,4 +1,5 @@
-// The autograd nodes of the attention ops and of the q / k prologue in C++, over
+// The autograd nodes of the attention ops and of the q / k prologue, and the launch of a
+// cached step whose arguments need no conversion, in C++, over
 // the C ABI of libmi_attn.so (include/mi_attn.h). flash_cuda.py and prologue.py
 // validate, cast and call these; the kernels' arguments, outputs and saved
 // tensors are the same as before.
@@ -9,11 +10,14 @@
 // small training step is bound by that host path: forward + backward of a small
 // attention call 118 -> 74 us, of a small prologue 122 -> 62 us (one box, medians;
 // torch's own `mul` takes 55 us forward + backward there). A call that a tracer
-// records keeps the Python nodes (flash_cuda._python_node).
+// records keeps the Python nodes (flash_cuda._python_node). A cached step is bound by the
+// host the same way: decode.attn_tree 18.5 -> 9.1 us, tree_commit 15.6 -> 6.2 us a call.
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -21,6 +25,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
 
 #include "../../include/mi_attn.h"
 
@@ -377,6 +383,166 @@ PyObject* py_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// Cached steps, for arguments that need no conversion. These return None for anything
+// else, refusals included: decode.py then converts, or says what is wrong.
+// ---------------------------------------------------------------------------
+bool plain_arg(PyObject* o, Tensor& out) {      // a Tensor itself, or None
+  if (o == Py_None) return true;
+  if (!THPVariable_CheckExact(o)) return false;
+  out = THPVariable_Unpack(o);
+  return true;
+}
+
+bool kernel_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+// A dense tensor of `dtype` on q's device with these sizes.
+bool dense_like(const Tensor& t, const Tensor& q, at::ScalarType dtype, at::IntArrayRef sizes) {
+  return t.defined() && t.scalar_type() == dtype && t.device() == q.device() && t.sizes() == sizes &&
+         t.is_contiguous();
+}
+
+// Cache rows as the kernels read them: D apart, strides and address in 16-byte chunks.
+bool cache_ok(const Tensor& t, const Tensor& k) {
+  if (!t.defined() || t.dim() != 4 || t.scalar_type() != k.scalar_type() || t.device() != k.device())
+    return false;
+  const int64_t D = k.size(3), chunk = 16 / t.element_size();
+  return t.size(0) == k.size(0) && t.size(1) == k.size(2) && t.size(3) == D && t.stride(3) == 1 &&
+         t.stride(2) == D && t.stride(0) % chunk == 0 && t.stride(1) % chunk == 0 &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+bool tracked(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// Whether k, v [B,T,Hkv,D] are what the kernels read, on the current device, with nothing
+// for autograd or autocast to do.
+bool block_ok(const Tensor& k, const Tensor& v) {
+  if (!k.defined() || k.dim() != 4 || !k.is_cuda() || !kernel_type(k.scalar_type()) || !k.is_contiguous())
+    return false;
+  if (!dense_like(v, k, k.scalar_type(), k.sizes())) return false;
+  const int64_t D = k.size(3);
+  if ((D != 32 && D != 64 && D != 128) || k.size(2) == 0) return false;
+  if (k.get_device() != c10::hip::current_device() || at::autocast::is_autocast_enabled(at::kCUDA)) return false;
+  return !at::GradMode::is_enabled() || (!tracked(k) && !tracked(v));
+}
+
+bool fits_int(int64_t n) { return n <= 0x7fffffff; }
+
+mi_step_shape step_shape(const Tensor& q, const Tensor& k, const Tensor& ck, const Tensor& cv) {
+  mi_step_shape s = {};
+  s.B = static_cast<int>(k.size(0));
+  s.T = static_cast<int>(k.size(1));
+  s.H = static_cast<int>(q.size(2));
+  s.Hkv = static_cast<int>(k.size(2));
+  s.D = static_cast<int>(k.size(3));
+  s.maps = 1;
+  s.scale = 1.f;
+  s.dtype = code_of(k);
+  if (ck.defined()) {
+    s.rows = static_cast<int>(ck.size(2));
+    s.k_batch_stride = ck.stride(0);
+    s.k_head_stride = ck.stride(1);
+    s.v_batch_stride = cv.stride(0);
+    s.v_head_stride = cv.stride(1);
+  }
+  return s;
+}
+
+// step(q, k, v, cache k, cache v, lens, parents, lam, gate, causal, scale, return_lse)
+// -> out, (out, lse) or None.
+PyObject* py_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, ck, cv, lens, parents, lam, gate;
+  TORCH_CHECK_TYPE(n == 12, "step(q, k, v, cache_k, cache_v, lens, parents, lam, gate, causal, scale, return_lse)");
+  if (!plain_arg(args[0], q) || !plain_arg(args[1], k) || !plain_arg(args[2], v) || !plain_arg(args[3], ck) ||
+      !plain_arg(args[4], cv) || !plain_arg(args[5], lens) || !plain_arg(args[6], parents) ||
+      !plain_arg(args[7], lam) || !plain_arg(args[8], gate))
+    Py_RETURN_NONE;
+  const int64_t causal = PyObject_IsTrue(args[9]), want_lse = PyObject_IsTrue(args[11]);
+  double scale = 0.0;
+  if (args[10] != Py_None) scale = PyFloat_AsDouble(args[10]);
+  if (PyErr_Occurred()) throw python_error();
+  if (!q.defined() || q.dim() != 4 || !block_ok(k, v) || ck.defined() != cv.defined()) Py_RETURN_NONE;
+  const int64_t B = k.size(0), T = k.size(1), Hkv = k.size(2), D = k.size(3), H = q.size(2);
+  if (!dense_like(q, k, k.scalar_type(), {B, T, H, D}) || H % Hkv) Py_RETURN_NONE;
+  if (ck.defined() && (!cache_ok(ck, k) || !cache_ok(cv, k) || ck.size(2) != cv.size(2) || !fits_int(ck.size(2))))
+    Py_RETURN_NONE;
+  if (lens.defined() && !dense_like(lens, k, at::kInt, {B})) Py_RETURN_NONE;
+  const bool one_tree = parents.defined() && parents.dim() == 1;
+  if (parents.defined() && (T > MI_TREE_MAX || !(one_tree ? dense_like(parents, k, at::kInt, {T})
+                                                          : dense_like(parents, k, at::kInt, {B, T}))))
+    Py_RETURN_NONE;
+  if (lam.defined() && (want_lse || !kernel_type(lam.scalar_type()) || !dense_like(lam, k, lam.scalar_type(), {H})))
+    Py_RETURN_NONE;
+  if (gate.defined() && !dense_like(gate, k, at::kFloat, {B, T, H})) Py_RETURN_NONE;
+  if (at::GradMode::is_enabled() && (tracked(q) || tracked(lam) || tracked(gate))) Py_RETURN_NONE;
+  if (args[10] == Py_None) scale = std::sqrt((lam.defined() ? 2.0 : 1.0) / static_cast<double>(D));
+  if (!std::isfinite(scale) || !(scale > 0.0) || !fits_int(B) || !fits_int(T) || !fits_int(H)) Py_RETURN_NONE;
+  mi_step_shape s = step_shape(q, k, ck, cv);
+  s.causal = static_cast<int>(causal);
+  s.one_tree = one_tree;
+  s.scale = static_cast<float>(scale);
+  if (lam.defined()) {
+    s.maps = 2;
+    s.lam_dtype = code_of(lam);
+  }
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard no_grad;
+    long long floats_ws = 0;
+    check(mi_attn_step_workspace(&s, &floats_ws));
+    out = at::empty_like(q);
+    // From torch's allocator at every call: a captured graph gets one of its own.
+    const Tensor ws = floats_ws ? at::empty({static_cast<int64_t>(floats_ws)}, q.options().dtype(at::kFloat))
+                                : Tensor();
+    if (want_lse) lse = at::empty({B, H, T}, q.options().dtype(at::kFloat));
+    check(mi_attn_step(ptr(q), ptr(k), ptr(v), ptr(ck), ptr(cv), static_cast<const int*>(ptr(lens)),
+                       static_cast<const int*>(ptr(parents)), ptr(lam), floats(gate), ptr(out), floats(lse),
+                       floats(ws), &s, stream_of(q)));
+  }
+  PyObject* o = THPVariable_Wrap(std::move(out));
+  if (!o) throw python_error();
+  if (!want_lse) return o;
+  PyObject* l = THPVariable_Wrap(std::move(lse));
+  PyObject* t = l ? PyTuple_Pack(2, o, l) : nullptr;
+  Py_DECREF(o);
+  Py_XDECREF(l);
+  if (!t) throw python_error();
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// tree_commit(k, v, cache k, cache v, lens, path, count) -> the new lens or None.
+PyObject* py_tree_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor k, v, ck, cv, lens, path, count;
+  TORCH_CHECK_TYPE(n == 7, "tree_commit(k, v, cache_k, cache_v, lens, path, count)");
+  if (!plain_arg(args[0], k) || !plain_arg(args[1], v) || !plain_arg(args[2], ck) || !plain_arg(args[3], cv) ||
+      !plain_arg(args[4], lens) || !plain_arg(args[5], path) || !plain_arg(args[6], count))
+    Py_RETURN_NONE;
+  if (!block_ok(k, v) || !cache_ok(ck, k) || !cache_ok(cv, k) || ck.size(2) != cv.size(2)) Py_RETURN_NONE;
+  const int64_t B = k.size(0);
+  if (!path.defined() || path.dim() != 2) Py_RETURN_NONE;
+  const int64_t P = path.size(1);
+  if (!dense_like(lens, k, at::kInt, {B}) || !dense_like(path, k, at::kInt, {B, P}) ||
+      !dense_like(count, k, at::kInt, {B}) || !fits_int(B) || !fits_int(k.size(1)) || !fits_int(P) ||
+      !fits_int(ck.size(2)))
+    Py_RETURN_NONE;
+  const mi_step_shape s = step_shape(k, k, ck, cv);
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::NoGradGuard no_grad;
+    out = at::empty_like(lens);
+    check(mi_attn_tree_commit(ptr(k), ptr(v), ptr(ck), ptr(cv), static_cast<const int*>(ptr(lens)),
+                              static_cast<const int*>(ptr(path)), static_cast<const int*>(ptr(count)),
+                              static_cast<int*>(ptr(out)), static_cast<int>(P), &s, stream_of(k)));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_attn)), METH_FASTCALL,
      "attn(q, k, v, gate, causal, window, sinks, scale, block, residual) -> (O, LSE)"},
@@ -384,6 +550,10 @@ PyMethodDef methods[] = {
      "prologue(x, weight, cos, sin, eps, out_dtype) -> out"},
     {"diff_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_diff_attn)), METH_FASTCALL,
      "diff_attn(q, k, v, lam, causal, scale) -> out"},
+    {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_step)), METH_FASTCALL,
+     "step(q, k, v, cache_k, cache_v, lens, parents, lam, gate, causal, scale, return_lse) -> out, (out, lse) or None"},
+    {"tree_commit", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_tree_commit)), METH_FASTCALL,
+     "tree_commit(k, v, cache_k, cache_v, lens, path, count) -> lens or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mi_torch", nullptr, -1, methods, nullptr, nullptr,

@@ -889,6 +889,11 @@ int validate_step(const mi_step_shape* s) {
   if ((long long)s->B * s->T * s->H > 0x7fffffffLL) return MI_ERR_SIZE;
   if (32LL * s->Hkv * s->D * 4 > 0x7fffffffLL) return MI_ERR_SIZE;
   if ((long long)s->rows + s->T > 0x7fffff00LL) return MI_ERR_SIZE;
+  // 32-key blocks of every unit (at least 32 query rows), with 16 more for each.
+  const long long rep = s->Hkv > 0 ? s->H / s->Hkv : 1;
+  if ((long long)s->B * s->Hkv * ((s->T * rep + 31) / 32) * (((long long)s->rows + s->T + 62) / 32 + 16) >
+      0x7fffffffLL)
+    return MI_ERR_SIZE;
   return MI_OK;
 }
 

@@ -382,9 +382,14 @@ def _whole_numbers(t, shapes, dev, who, name, top):
 
 
 def _step(who, q, k, v, dims, cache, parents, causal, lam, scale, gate, return_lse):
-    """One launch of ``mi_attn_step`` over ``cache``; q, k, v as the caller gave them."""
+    """One launch of ``mi_attn_step`` over ``cache``; q, k, v as the caller gave them. (The
+    extension's ``step`` is the same for arguments that need no conversion.)"""
     B, T, H, Hkv, D, dtype = dims
     dev = q.device
+    if parents is None and who == "attn_tree":
+        raise ValueError(f"{who}: parents must be an int32 or int64 tensor, got None")
+    if lam is None and who == "diff_attn_cached":
+        raise ValueError(f"{who}: lam must be a tensor, got None")
     if k.device != dev or v.device != dev:
         raise ValueError(f"{who}: q, k and v must be on one device, got {dev}, {k.device}, {v.device}")
     scale = math.sqrt((1 if lam is None else 2) / D) if scale is None else float(scale)
@@ -464,9 +469,14 @@ def attn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict,
     output, and the (B, H, T) float32 LSE too when ``return_lse`` (one map only).
     """
     who = "attn_tree"
-    dims = _check_block(q, k, v, who)
     if "pos" in cache:
         raise ValueError(f"{who}: a windowed cache ('pos') holds no draft trees")
+    if _fc._ext is not None and parents is not None:     # arguments that need no conversion
+        out = _fc._ext.step(q, k, v, cache.get("k"), cache.get("v"), cache.get("lens"), parents,
+                            lam, gate, True, scale, return_lse)
+        if out is not None:
+            return out
+    dims = _check_block(q, k, v, who)
     return _step(who, q, k, v, dims, cache, parents, True, lam, scale, gate, return_lse)
 
 
@@ -478,13 +488,19 @@ def diff_attn_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: tor
     or one value; ``scale`` defaults to 1/sqrt(E/2). Returns the (B, T, H, E) output.
     """
     who = "diff_attn_cached"
-    dims = _check_block(q, k, v, who)
     for name in ("lens", "pos"):
         if name in cache:
             raise ValueError(f"{who}: the cache holds {name!r}: "
                              + ("a length for each sequence, attn_tree's" if name == "lens"
                                 else "a window's, which differential attention has not"))
-    out = _step(who, q, k, v, dims, cache, None, causal, lam, scale, gate, False)
+    out = None
+    if _fc._ext is not None and lam is not None:
+        out = _fc._ext.step(q, k, v, cache.get("k"), cache.get("v"), None, None, lam, gate, causal,
+                            scale, False)
+    if out is None or commit:
+        dims = _check_block(q, k, v, who)
+    if out is None:
+        out = _step(who, q, k, v, dims, cache, None, causal, lam, scale, gate, False)
     if commit:
         T, dtype, dev = dims[1], dims[5], q.device
         for name, held, new in (("k", _KBUF, k), ("v", _VBUF, v)):
@@ -536,6 +552,12 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, cache: dict, path: torch.Tenso
     past it are dropped. A node outside [0, T) leaves its row as it was.
     """
     who = "tree_commit"
+    if _fc._ext is not None:                             # arguments that need no conversion
+        new = _fc._ext.tree_commit(k, v, cache.get("k"), cache.get("v"), cache.get("lens"), path,
+                                   count)
+        if new is not None:
+            cache["lens"] = new
+            return
     B, T, _, Hkv, D, dtype = _check_block(k, k, v, who)
     dev = k.device
     for name in ("k", "v"):

@@ -603,6 +603,8 @@ def _lam_of(lam, q, who):
     if lam.device != q.device or lam.dim() > 1 or (lam.numel() != H and lam.numel() != 1):
         raise ValueError(f"{who}: lam must be [H] = [{H}] or one value for every head, on "
                          f"{q.device}; got {tuple(lam.shape)} on {lam.device}")
+    if lam.dim() == 1 and lam.shape[0] == H and lam.is_contiguous():
+        return lam                     # no views for autograd to record
     return lam.reshape(-1).expand(H).contiguous()
 
 

@@ -224,6 +224,8 @@ def test_refusals():
     refused("parents must be", tree, q, k, v, cache, up.float())
     refused("parents must be", tree, q, k, v, cache, up.cpu())
     refused("parents must be", tree, q, k, v, cache, [-1, 0, 1])
+    refused("parents must be", tree, q, k, v, cache, None)
+    refused("lam must be", dec.diff_attn_cached, q, k, v, None, {}, False)
     refused("lens'\\] must be", tree, q, k, v, {**cache, "lens": lens[:1]}, up)
     refused("lens'\\] must be", tree, q, k, v, {**cache, "lens": lens.float()}, up)
     refused("only one of", tree, q, k, v, {"k": ck}, up)
@@ -490,6 +492,33 @@ def test_speculative_rounds(two):
         held = [(torch.cat([hk, k[b, x]]), torch.cat([hv, v[b, x]]))
                 for b, ((hk, hv), x) in enumerate(zip(held, take))]
         assert cache["lens"].tolist() == [h[0].shape[0] for h in held]
+
+
+@gpu
+def test_the_python_path_gives_the_same_bits(monkeypatch):
+    """Arguments that need no conversion are launched by the C++ extension, any others (and all
+    of them without it) by decode.py."""
+    assert fc._load() is not None and fc._ext is not None
+    q, k, v, ck, cv, lam = (t.cuda() for t in draw(3, 10, 4, 2, 64, 90, torch.bfloat16, seed=2))
+    cache = {"k": ck, "v": cv, "lens": torch.tensor([90, 4, 31], dtype=torch.int32, device="cuda")}
+    up = draft(3, 10, 1, pad=True).cuda()
+    gate = torch.randn(3, 10, 4, device="cuda")
+    path = torch.randint(0, 10, (3, 3), device="cuda", dtype=torch.int32)
+    count = torch.tensor([0, 3, 1], device="cuda", dtype=torch.int32)
+
+    def everything():
+        mine = {n: t.clone() for n, t in cache.items()}
+        out = [*dec.attn_tree(q, k, v, mine, up, return_lse=True),
+               dec.attn_tree(q, k, v, mine, up[0], lam=lam, gate=gate, scale=0.3),
+               dec.diff_attn_cached(q, k, v, lam, {"k": ck, "v": cv}, False, True),
+               dec.diff_attn_cached(q, k, v, lam, {}, False, gate=gate)]
+        dec.tree_commit(k, v, mine, path, count)
+        return out + [mine[n] for n in ("k", "v", "lens")]
+    fast = everything()
+    for call in ("step", "tree_commit"):
+        assert getattr(fc._ext, call) is not None
+    monkeypatch.setattr(fc, "_ext", None)
+    assert all(torch.equal(a, b) for a, b in zip(fast, everything()))
 
 
 @gpu
