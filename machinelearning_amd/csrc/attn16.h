@@ -148,6 +148,36 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// Per-lane byte offsets of the DMA lane map of a 64-row tile with row
+// stride `rs` elements, shared by NW waves: instruction j of wave w fills LDS
+// slots (NW j + w)*64 + lane, i.e. row slot / CH, physical chunk slot % CH.
+template <int D, int NW = 4>
+__device__ __forceinline__ void dma_offsets(unsigned (&voff)[D / 8 / NW], int wave, int lane,
+                                            long long rs) {
+  constexpr int CH = D / 8;   // 16-byte chunks per row
+#pragma unroll
+  for (int j = 0; j < CH / NW; ++j) {
+    const int slot = (NW * j + wave) * 64 + lane;
+    const int row = slot / CH;
+    voff[j] = (unsigned)(row * rs + ((slot % CH) ^ swz<D>(row)) * 8) * 2u;
+  }
+}
+
+// Transposed-read base offsets: for output tile dt (32 columns of the tile),
+// lane (G = lane >> 4, m = lane & 15) reads rows 4*(G>>1) + (m>>2) + 8h (+ 32mt
+// + 16ks as immediates), columns dt*32 + 16*(G&1) + 4*(m&3).
+template <int D>
+__device__ __forceinline__ void tr_offsets(int (&toff)[D / 32][2], int lane) {
+  const int G = lane >> 4, m = lane & 15;
+  const int row = 4 * (G >> 1) + (m >> 2);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    const int col = dt * 32 + 16 * (G & 1) + 4 * (m & 3);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) toff[dt][hh] = tile_off<D>(row + 8 * hh, col >> 3) + (col & 7) * 2;
+  }
+}
+
 // 8 consecutive 16-bit elements of one row (ds_read_b128).
 template <typename T>
 __device__ __forceinline__ typename Mfma32<T>::frag lds_frag(const char* p) {

@@ -42,36 +42,6 @@ struct Bwd16 {
   static constexpr int DS = D / 16, DT = D / 32;
 };
 
-// Per-lane byte offsets of the DMA lane map of a 64-row tile with row
-// stride `rs` elements, shared by NW waves: instruction j of wave w fills LDS
-// slots (NW j + w)*64 + lane, i.e. row slot / CH, physical chunk slot % CH.
-template <int D, int NW = 4>
-__device__ __forceinline__ void dma_offsets(unsigned (&voff)[Bwd16<D>::CH / NW], int wave, int lane,
-                                            long long rs) {
-  using C = Bwd16<D>;
-#pragma unroll
-  for (int j = 0; j < C::CH / NW; ++j) {
-    const int slot = (NW * j + wave) * 64 + lane;
-    const int row = slot / C::CH;
-    voff[j] = (unsigned)(row * rs + ((slot % C::CH) ^ swz<D>(row)) * 8) * 2u;
-  }
-}
-
-// Transposed-read base offsets: for output tile dt (32 columns of the tile),
-// lane (G = lane >> 4, m = lane & 15) reads rows 4*(G>>1) + (m>>2) + 8h (+ 32mt
-// + 16ks as immediates), columns dt*32 + 16*(G&1) + 4*(m&3).
-template <int D>
-__device__ __forceinline__ void tr_offsets(int (&toff)[Bwd16<D>::DT][2], int lane) {
-  const int G = lane >> 4, m = lane & 15;
-  const int row = 4 * (G >> 1) + (m >> 2);
-#pragma unroll
-  for (int dt = 0; dt < Bwd16<D>::DT; ++dt) {
-    const int col = dt * 32 + 16 * (G & 1) + 4 * (m & 3);
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) toff[dt][hh] = tile_off<D>(row + 8 * hh, col >> 3) + (col & 7) * 2;
-  }
-}
-
 template <int N>
 __device__ __forceinline__ void wait_ring(int n) {
   if (n <= 0) wait_vm<0>();

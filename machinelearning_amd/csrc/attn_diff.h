@@ -30,9 +30,7 @@ struct DiffParams {
   int wi_blocks_fastest;
 };
 
-// Planes of [B, H, S] floats: the forward's LSE of map m, and in the backward's
-// workspace delta of map m; after those, partial sums of delta_2 over `nblk` row
-// blocks of each (b, h).
+// A plane of [B, H, S] floats: the forward's LSE of each map, the backward's row values.
 __host__ __device__ inline long long diff_plane(const DiffParams& p) { return (long long)p.B * p.H * p.S; }
 
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, long long i) {
@@ -49,5 +47,9 @@ __device__ __forceinline__ void store_from_float(void* p, int dtype, long long i
     default: static_cast<__bf16*>(p)[i] = (__bf16)x;
   }
 }
+
+// dlam_h = -sum of delta_2 over h's rows, from its sums over `nblk` row blocks of each
+// (b, h) (attn_diff.hip).
+void launch_diff_dlam(const float* parts, int nblk, const DiffParams& p, hipStream_t st);
 
 }  // namespace mi

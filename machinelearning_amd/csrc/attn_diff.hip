@@ -1,4 +1,4 @@
-// Differential attention (attn_diff.h's formulas) for every dtype: forward, delta, dQ
+// Differential attention (attn_diff.h's formulas) in float32: forward, delta, dQ
 // and dK/dV, on [B,S,H,E] / [B,S,Hkv,E] tensors with native GQA.
 //
 // The walk is flash attention's: a workgroup of four waves owns 128 rows, a wave 32;
@@ -542,39 +542,45 @@ hipError_t diff_bwd_t(const void* q, const void* k, const void* v, const void* o
                      (const T*)dout, lse, ws, (T*)dq, p);
   hipLaunchKernelGGL((diff_dkdv_kernel<T, E>), keys, dim3(256), 0, st, (const T*)q, (const T*)k,
                      (const T*)v, (const T*)dout, lse, ws, (T*)dk, (T*)dv, p);
-  hipLaunchKernelGGL(diff_dlam_kernel, dim3((unsigned)p.H), dim3(256), 0, st, ws + 2 * diff_plane(p),
-                     p.nblk, p);
+  launch_diff_dlam(ws + 2 * diff_plane(p), p.nblk, p, st);
   return hipGetLastError();
 }
 
 template <typename F>
-hipError_t by_type(int dtype, int E, F f) {
-  const auto by_dim = [&](auto t) {
-    switch (E) {
-      case 32: return f(t, std::integral_constant<int, 32>{});
-      case 64: return f(t, std::integral_constant<int, 64>{});
-      case 128: return f(t, std::integral_constant<int, 128>{});
-    }
-    return hipErrorInvalidValue;
-  };
-  switch (dtype) {
-    case 0: return by_dim(float{});
-    case 1: return by_dim(_Float16{});
-    case 2: return by_dim(__bf16{});
+hipError_t by_dim(int E, F f) {
+  switch (E) {
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
   }
   return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-long long diff_workspace_floats(const DiffParams& p) {
+void launch_diff_dlam(const float* parts, int nblk, const DiffParams& p, hipStream_t st) {
+  hipLaunchKernelGGL(diff_dlam_kernel, dim3((unsigned)p.H), dim3(256), 0, st, parts, nblk, p);
+}
+
+// 16-bit inputs (attn_diff16.hip).
+long long diff16_workspace_floats(const DiffParams& p);
+hipError_t launch_diff16_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,
+                             void* o2, float* lse, const DiffParams& p, hipStream_t st);
+hipError_t launch_diff16_bwd(int dtype, int E, const void* q, const void* k, const void* v,
+                             const void* o, const void* o2, const void* dout, const float* lse,
+                             float* ws, void* dq, void* dk, void* dv, const DiffParams& p,
+                             hipStream_t st);
+
+long long diff_workspace_floats(int dtype, const DiffParams& p) {
+  if (dtype != 0) return diff16_workspace_floats(p);
   return 2 * diff_plane(p) + (long long)p.B * p.H * ((p.S + 127) / 128);
 }
 
 hipError_t launch_diff_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,
                            void* o2, float* lse, const DiffParams& p, hipStream_t st) {
-  return by_type(dtype, E, [&](auto t, auto e) {
-    return diff_fwd_t<decltype(t), decltype(e)::value>(q, k, v, o, o2, lse, p, st);
+  if (dtype != 0) return launch_diff16_fwd(dtype, E, q, k, v, o, o2, lse, p, st);
+  return by_dim(E, [&](auto e) {
+    return diff_fwd_t<float, decltype(e)::value>(q, k, v, o, o2, lse, p, st);
   });
 }
 
@@ -582,8 +588,9 @@ hipError_t launch_diff_bwd(int dtype, int E, const void* q, const void* k, const
                            const void* o, const void* o2, const void* dout, const float* lse,
                            float* ws, void* dq, void* dk, void* dv, const DiffParams& p,
                            hipStream_t st) {
-  return by_type(dtype, E, [&](auto t, auto e) {
-    return diff_bwd_t<decltype(t), decltype(e)::value>(q, k, v, o, o2, dout, lse, ws, dq, dk, dv, p, st);
+  if (dtype != 0) return launch_diff16_bwd(dtype, E, q, k, v, o, o2, dout, lse, ws, dq, dk, dv, p, st);
+  return by_dim(E, [&](auto e) {
+    return diff_bwd_t<float, decltype(e)::value>(q, k, v, o, o2, dout, lse, ws, dq, dk, dv, p, st);
   });
 }
 

@@ -73,7 +73,7 @@ hipError_t launch_prologue_bwd(int dtype_in, int dtype_out, int D, const void* g
                                const float* w, const float* cs, const float* sn,
                                const float* rstd, void* dx, float* dw, float* part,
                                const ProParams& p, hipStream_t st);
-long long diff_workspace_floats(const DiffParams& p);
+long long diff_workspace_floats(int dtype, const DiffParams& p);
 hipError_t launch_diff_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,
                            void* o2, float* lse, const DiffParams& p, hipStream_t st);
 hipError_t launch_diff_bwd(int dtype, int E, const void* q, const void* k, const void* v,
@@ -853,7 +853,7 @@ int mi_attn_diff_bwd_workspace(const mi_diff_shape* s, long long* floats) {
   if (!floats) return MI_ERR_NULL;
   const int st = validate_diff(s);
   if (st) return st;
-  *floats = empty_diff(s) ? 0 : mi::diff_workspace_floats(diff_params(s, nullptr, nullptr));
+  *floats = empty_diff(s) ? 0 : mi::diff_workspace_floats(s->dtype, diff_params(s, nullptr, nullptr));
   return MI_OK;
 }
 
