@@ -28,6 +28,9 @@ struct DiffParams {
   void* dlam;             // [H], of lam_dtype
   FastDiv div_h, div_hkv, div_group, div_wi;
   int wi_blocks_fastest;
+  // 16-bit dK/dV dealt evenly (diff16_dkdv_kernel): steps of the whole line, of one (batch,
+  // kv head) and of one workgroup; 0: a workgroup per key block.
+  int line_n, line_head, line_per;
 };
 
 // A plane of [B, H, S] floats: the forward's LSE of each map, the backward's row values.
@@ -48,8 +51,20 @@ __device__ __forceinline__ void store_from_float(void* p, int dtype, long long i
   }
 }
 
-// dlam_h = -sum of delta_2 over h's rows, from its sums over `nblk` row blocks of each
-// (b, h) (attn_diff.hip).
-void launch_diff_dlam(const float* parts, int nblk, const DiffParams& p, hipStream_t st);
+// dlam_h = -sum of delta_2 over h's rows, from its sums over p.nblk row blocks of each
+// (b, h): by the last workgroups of a launch of 256 threads, a head each. `lds`: four floats.
+__device__ __forceinline__ void reduce_dlam(const float* __restrict__ sums, float* lds, const DiffParams& p) {
+  const int tid = threadIdx.x;
+  for (int h = (int)(gridDim.x - 1 - blockIdx.x); h < p.H; h += (int)gridDim.x) {
+    float x = 0.f;
+    for (int i = tid; i < p.B * p.nblk; i += 256) x += sums[((long long)(i / p.nblk) * p.H + h) * p.nblk + i % p.nblk];
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    if ((tid & 63) == 0) lds[tid >> 6] = x;
+    __syncthreads();
+    if (tid == 0) store_from_float(p.dlam, p.lam_dtype, h, -((lds[0] + lds[1]) + (lds[2] + lds[3])));
+    __syncthreads();
+  }
+}
 
 }  // namespace mi

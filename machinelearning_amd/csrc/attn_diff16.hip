@@ -461,12 +461,44 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
 //   S'_m = q_m k_m^T - L_m / scale   -> p_m = exp2(c S'_m)
 //   G'   = dO (-V)^T + delta_1       -> p_1 G' = -dS_1
 //   lam G' + lam (delta_2 - delta_1) -> p_2 times that = dS_2
+//
+// LINE: where the key blocks are few, a workgroup each leaves the chip half idle (causal
+// blocks differ up to S / 64-fold, and a kv head's block walks every head of its group). The
+// steps (group head, query tile) of all key blocks then form one line, block after block, cut
+// into equal pieces. A block that several pieces share gets float32 partials, at most two
+// slots a workgroup, which diff16_join_kernel adds in order. Each block has kLineSetup empty
+// steps in front: what starting one costs.
+//
+// The workgroups of the line's end (the lightest blocks') also reduce dlam.
 // ---------------------------------------------------------------------------
-template <typename T, int E>
+constexpr int kLineSetup = 3;
+
+// Steps of the line before key block i of its (batch, kv head), setups included.
+__host__ __device__ inline int line_before(const DiffParams& p, int i) {
+  const int NT = (p.S + 63) / 64;
+  return i * (p.group * NT + kLineSetup) - (p.causal ? p.group * i * (i - 1) : 0);
+}
+// The key block that step x of a (batch, kv head) belongs to.
+__device__ __forceinline__ int line_block(const DiffParams& p, int x) {
+  const int NT = (p.S + 63) / 64;
+  int i;
+  if (p.causal) {
+    const float a = (float)(p.group * NT + kLineSetup + p.group);
+    i = (int)((a - sqrtf(fmaxf(a * a - 4.f * p.group * (float)x, 0.f))) / (2.f * p.group));
+    i = __builtin_amdgcn_readfirstlane(max(0, min(i, p.nblk - 1)));
+    while (i > 0 && line_before(p, i) > x) --i;
+    while (i + 1 < p.nblk && line_before(p, i + 1) <= x) ++i;
+  } else {
+    i = x / (p.group * NT + kLineSetup);
+  }
+  return i;
+}
+
+template <typename T, int E, bool LINE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(E <= 64 ? 2 : 1, 8)))
 diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                    const T* __restrict__ dO, const float* __restrict__ ws, T* __restrict__ dK,
-                   T* __restrict__ dV, DiffParams p) {
+                   T* __restrict__ dV, float* __restrict__ part, DiffParams p) {
   using C = Diff16<E>;
   using M = Mfma32<T>;
   using frag = typename M::frag;
@@ -477,7 +509,31 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, g = lane >> 5;
-  const WorkItem wi = work_item(p.nblk, p.B * p.Hkv, p.div_wi, false, p.wi_blocks_fastest);
+  reduce_dlam(ws + kPlanes * diff_plane(p), vecs[0][0], p);
+  int at = 0, end = 1;
+  if constexpr (LINE) {
+    at = (int)blockIdx.x * p.line_per;
+    end = min(at + p.line_per, p.line_n);
+  }
+  const int begin = at;
+  do {
+  WorkItem wi;
+  int f0 = 0, f1 = 0x7fffffff, took = 1;
+  bool whole = true;
+  if constexpr (LINE) {
+    wi.bh = at / p.line_head;
+    const int x = at - wi.bh * p.line_head;
+    wi.blk = line_block(p, x);
+    const int start = line_before(p, wi.blk), from = x - start;
+    const int span = line_before(p, wi.blk + 1) - start, to = min(span, from + end - at);
+    f0 = max(from - kLineSetup, 0);
+    f1 = to - kLineSetup;
+    whole = f0 == 0 && to == span;
+    took = to - from;
+    if (f1 <= f0) break;                           // the piece ends in a block's empty steps
+  } else {
+    wi = work_item(p.nblk, p.B * p.Hkv, p.div_wi, false, p.wi_blocks_fastest);
+  }
   const int b = (int)fdiv((unsigned)wi.bh, p.div_hkv), hkv = wi.bh - b * p.Hkv;
   const int k0 = wi.blk * BK, kw0 = k0 + wave * 32, kj = kw0 + l32;
   const long long koff = (long long)b * p.S * p.kv_rs + (long long)hkv * E;
@@ -493,7 +549,7 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
     vf[ds] = __builtin_bit_cast(frag, bits);
   }
   const int tq_begin = p.causal ? k0 / BQ : 0, tq_end = (p.S + BQ - 1) / BQ;
-  const int niter = p.group * (tq_end - tq_begin);
+  const int ntq = tq_end - tq_begin, niter = LINE ? f1 - f0 : p.group * ntq;
   int tw_begin = tq_begin;
   if (p.causal) tw_begin = kw0 / BQ;
   if (kw0 >= p.S) tw_begin = tq_end;
@@ -504,10 +560,12 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
   const unsigned m0v = lds_u32(vecs[0][0] + wave * 16);
   const long long plane = diff_plane(p);
   // Issue position, one unit per issue; the head's descriptors follow its head.
-  int is_gh = 0, is_tq = tq_begin;
-  RowTiles tQ = row_tiles(Q, b, p.S, p.q_rs, hkv * p.group, E);
-  RowTiles tO = row_tiles(dO, b, p.S, p.q_rs, hkv * p.group, E);
-  const float* vec = ws + ((long long)b * p.H + hkv * p.group) * p.S;
+  const int gh0 = LINE ? f0 / ntq : 0;
+  int is_gh = gh0, is_tq = tq_begin + (LINE ? f0 - gh0 * ntq : 0);
+  int cp_tq = is_tq, cp_h = hkv * p.group + gh0;
+  RowTiles tQ = row_tiles(Q, b, p.S, p.q_rs, cp_h, E);
+  RowTiles tO = row_tiles(dO, b, p.S, p.q_rs, cp_h, E);
+  const float* vec = ws + ((long long)b * p.H + cp_h) * p.S;
   auto issue = [&](int slot) __attribute__((always_inline)) {
     const Rsrc rq = tile_rsrc(tQ, is_tq), ro = tile_rsrc(tO, is_tq);
 #pragma unroll
@@ -623,7 +681,6 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
     }
   };
 
-  int cp_tq = tq_begin, cp_h = hkv * p.group;
   float lam = load_as_float(p.lam, p.lam_dtype, cp_h);
   auto step = [&](auto slot_c, int it) __attribute__((always_inline)) {
     constexpr int SL = decltype(slot_c)::value;
@@ -656,9 +713,54 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
       const bool second = C::SHARED ? r >= 8 : dt >= DT / 2;
       out[dt][r] = dk[C::SHARED ? (int)second : dt][r] * (second ? p.scale : -p.scale);
     }
-  store_rows_lds<T, E>(out, 1.f, stage, dK + off, p.kv_rs, p.S - kw0, lane);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  store_rows_lds<T, E>(dv, 1.f, stage, dV + off, p.kv_rs, p.S - kw0, lane);
+  if (whole) {
+    store_rows_lds<T, E>(out, 1.f, stage, dK + off, p.kv_rs, p.S - kw0, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    store_rows_lds<T, E>(dv, 1.f, stage, dV + off, p.kv_rs, p.S - kw0, lane);
+  } else {
+    // This piece's share: [128 keys][dK | dV] floats.
+    float* dst = part + ((2LL * blockIdx.x + (at != begin)) * BK + wave * 32 + l32) * (2 * E);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d0 = dt * 32 + 8 * j + 4 * g;
+        *reinterpret_cast<f32x4*>(dst + d0) =
+            f32x4{out[dt][4 * j], out[dt][4 * j + 1], out[dt][4 * j + 2], out[dt][4 * j + 3]};
+        *reinterpret_cast<f32x4*>(dst + E + d0) =
+            f32x4{dv[dt][4 * j], dv[dt][4 * j + 1], dv[dt][4 * j + 2], dv[dt][4 * j + 3]};
+      }
+  }
+  at += took;
+  if constexpr (LINE) __syncthreads();             // the ring is free for the next block
+  } while (LINE && at < end);
+}
+
+// The key blocks that several pieces of the line share: their partials added in the line's
+// order. A thread per 8 elements of a key's dK or dV, `per_unit` workgroups a block.
+template <typename T, int E>
+__global__ void __launch_bounds__(256)
+diff16_join_kernel(const float* __restrict__ part, T* __restrict__ dK, T* __restrict__ dV, DiffParams p) {
+  constexpr int C8 = 2 * E / 8, PER_UNIT = 128 * C8 / 256;
+  const int u = blockIdx.x / PER_UNIT, x = (int)(blockIdx.x % PER_UNIT) * 256 + threadIdx.x;
+  const int bh = u / p.nblk, blk = u % p.nblk;
+  const int start = bh * p.line_head + line_before(p, blk), stop = bh * p.line_head + line_before(p, blk + 1);
+  const int g0 = (start + kLineSetup) / p.line_per, g1 = (stop - 1) / p.line_per;
+  if (g0 == g1) return;                            // written by the workgroup that had it all
+  const int row = x / C8, c = x % C8, kj = blk * 128 + row;
+  if (kj >= p.S) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, d = a;
+  for (int w = g0; w <= g1; ++w) {
+    // The first of them may have begun with another block.
+    const float* src = part + ((2LL * w + (start > w * p.line_per)) * 128 + row) * (2 * E) + c * 8;
+    a += *reinterpret_cast<const f32x4*>(src);
+    d += *reinterpret_cast<const f32x4*>(src + 4);
+  }
+  const bool is_v = c >= C8 / 2;
+  const int b = bh / p.Hkv, hkv = bh % p.Hkv;
+  T* dst = (is_v ? dV : dK) + ((long long)b * p.S + kj) * p.kv_rs + (long long)hkv * E + (c % (C8 / 2)) * 8;
+  st_quad<T>(dst, a[0], a[1], a[2], a[3]);
+  st_quad<T>(dst + 4, d[0], d[1], d[2], d[3]);
 }
 
 namespace {
@@ -674,6 +776,31 @@ hipError_t diff16_fwd_t(const void* q, const void* k, const void* v, void* o, vo
   return hipGetLastError();
 }
 
+// Whether dK/dV deals its steps evenly, and how: where a workgroup per key block fills the
+// chip's slots less than twice. Fills the line's fields.
+int line_slots(int E) { return E <= 64 ? 512 : 256; }
+
+void diff16_line(DiffParams& p, int E) {
+  p.line_n = p.line_head = p.line_per = 0;
+  const long long nblk = (p.S + 127) / 128, units = nblk * p.B * p.Hkv;
+  const long long NT = (p.S + 63) / 64;
+  const long long head = nblk * (p.group * NT + kLineSetup) - (p.causal ? p.group * nblk * (nblk - 1) : 0);
+  if (units >= 2LL * line_slots(E) || head * p.B * p.Hkv >= (1LL << 30) || p.group * NT >= (1LL << 24)) return;
+  p.line_head = (int)head;
+  p.line_n = (int)(head * p.B * p.Hkv);
+  const int per = (p.line_n + line_slots(E) - 1) / line_slots(E);
+  p.line_per = per < 6 ? 6 : per;
+}
+
+// Floats of the line's partials: two slots a workgroup.
+long long line_floats(const DiffParams& p, int E) {
+  return p.line_per ? 2LL * ((p.line_n + p.line_per - 1) / p.line_per) * 128 * 2 * E : 0;
+}
+// They follow the planes and the sums, 256-byte aligned.
+long long line_offset(const DiffParams& p) {
+  return (kPlanes * diff_plane(p) + (long long)p.B * p.H * ((p.S + 127) / 128) + 63) / 64 * 64;
+}
+
 template <typename T, int E>
 hipError_t diff16_bwd_t(const void* q, const void* k, const void* v, const void* o, const void* o2,
                         const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
@@ -686,9 +813,19 @@ hipError_t diff16_bwd_t(const void* q, const void* k, const void* v, const void*
                      lse, ws, (T*)dq, p);
   DiffParams pk = p;
   pk.div_wi = p.wi_blocks_fastest ? p.div_wi : work_item_div((long long)p.B * p.Hkv);
-  hipLaunchKernelGGL((diff16_dkdv_kernel<T, E>), dim3((unsigned)((long long)p.nblk * p.B * p.Hkv)), dim3(256),
-                     0, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout, ws, (T*)dk, (T*)dv, pk);
-  launch_diff_dlam(ws + kPlanes * diff_plane(p), p.nblk, p, st);
+  diff16_line(pk, E);
+  const unsigned units = (unsigned)((long long)p.nblk * p.B * p.Hkv);
+  float* part = ws + line_offset(p);
+  if (pk.line_per) {
+    hipLaunchKernelGGL((diff16_dkdv_kernel<T, E, true>), dim3((pk.line_n + pk.line_per - 1) / pk.line_per),
+                       dim3(256), 0, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout, ws, (T*)dk,
+                       (T*)dv, part, pk);
+    hipLaunchKernelGGL((diff16_join_kernel<T, E>), dim3(units * (128 * 2 * E / 8 / 256)), dim3(256), 0, st,
+                       part, (T*)dk, (T*)dv, pk);
+  } else {
+    hipLaunchKernelGGL((diff16_dkdv_kernel<T, E, false>), dim3(units), dim3(256), 0, st, (const T*)q,
+                       (const T*)k, (const T*)v, (const T*)dout, ws, (T*)dk, (T*)dv, part, pk);
+  }
   return hipGetLastError();
 }
 
@@ -707,8 +844,10 @@ hipError_t by_type(int dtype, int E, F f) {
 
 }  // namespace
 
-long long diff16_workspace_floats(const DiffParams& p) {
-  return kPlanes * diff_plane(p) + (long long)p.B * p.H * ((p.S + 127) / 128);
+long long diff16_workspace_floats(const DiffParams& p, int E) {
+  DiffParams l = p;
+  diff16_line(l, E);
+  return line_offset(p) + line_floats(l, E);
 }
 
 hipError_t launch_diff16_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,

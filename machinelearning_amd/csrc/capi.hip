@@ -73,7 +73,7 @@ hipError_t launch_prologue_bwd(int dtype_in, int dtype_out, int D, const void* g
                                const float* w, const float* cs, const float* sn,
                                const float* rstd, void* dx, float* dw, float* part,
                                const ProParams& p, hipStream_t st);
-long long diff_workspace_floats(int dtype, const DiffParams& p);
+long long diff_workspace_floats(int dtype, int E, const DiffParams& p);
 hipError_t launch_diff_fwd(int dtype, int E, const void* q, const void* k, const void* v, void* o,
                            void* o2, float* lse, const DiffParams& p, hipStream_t st);
 hipError_t launch_diff_bwd(int dtype, int E, const void* q, const void* k, const void* v,
@@ -805,7 +805,11 @@ int validate_diff(const mi_diff_shape* s) {
   if (!s) return MI_ERR_NULL;
   if (s->lam_dtype != MI_F32 && s->lam_dtype != MI_F16 && s->lam_dtype != MI_BF16) return MI_ERR_DTYPE;
   const mi_attn_shape a = {s->B, s->S, s->H, s->Hkv, s->E, s->causal, 0, s->scale, s->dtype, 0, 0};
-  return validate(&a);
+  const int st = validate(&a);
+  if (st) return st;
+  // The float32 kernels' offsets within a sequence are 32-bit bytes.
+  if (s->dtype == MI_F32 && (s->S + 32LL) * s->H * s->E > 0x1fffffffLL) return MI_ERR_SIZE;
+  return MI_OK;
 }
 
 mi::DiffParams diff_params(const mi_diff_shape* s, const void* lam, void* dlam) {
@@ -830,6 +834,7 @@ mi::DiffParams diff_params(const mi_diff_shape* s, const void* lam, void* dlam) 
   p.div_group = mi::fast_div((unsigned)p.group);
   p.div_wi = mi::fast_div(1);   // set by each launcher for its grid
   p.wi_blocks_fastest = 0;
+  p.line_n = p.line_head = p.line_per = 0;
   return p;
 }
 
@@ -853,7 +858,7 @@ int mi_attn_diff_bwd_workspace(const mi_diff_shape* s, long long* floats) {
   if (!floats) return MI_ERR_NULL;
   const int st = validate_diff(s);
   if (st) return st;
-  *floats = empty_diff(s) ? 0 : mi::diff_workspace_floats(s->dtype, diff_params(s, nullptr, nullptr));
+  *floats = empty_diff(s) ? 0 : mi::diff_workspace_floats(s->dtype, s->E, diff_params(s, nullptr, nullptr));
   return MI_OK;
 }
 

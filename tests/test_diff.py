@@ -134,7 +134,7 @@ def diff_shape(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(B=-1), 2), (dict(S=-1), 2), (dict(H=3, Hkv=2), 2), (dict(Hkv=0), 2), (dict(E=48), 4),
     (dict(E=256), 4), (dict(dtype=7), 3), (dict(lam_dtype=-1), 3), (dict(scale=0.0), 9),
-    (dict(scale=float("nan")), 9), (dict(scale=float("inf")), 9), (dict(S=1 << 25, H=64), 7)])
+    (dict(scale=float("nan")), 9), (dict(scale=float("inf")), 9), (dict(S=1 << 25, H=64), 7), (dict(S=1 << 24, dtype=_capi.MI_F32), 7)])
 def test_abi_refuses_shapes(kw, code):
     lib, s, n = _capi.load(), diff_shape(**kw), ctypes.c_longlong(-1)
     assert lib.mi_attn_diff_bwd_workspace(ctypes.byref(s), ctypes.byref(n)) == code
@@ -212,7 +212,9 @@ def test_lengths(E, dtype, causal):
 @pytest.mark.parametrize("B,S,H,Hkv,E,causal", [
     (2, 300, 4, 4, 64, True), (3, 257, 6, 2, 32, True), (1, 700, 8, 1, 128, True),
     (8, 130, 8, 8, 64, False), (2, 513, 12, 4, 64, True), (5, 77, 9, 3, 32, False),
-    (1, 1500, 2, 2, 128, False)])
+    (1, 1500, 2, 2, 128, False),
+    # Enough key blocks for a workgroup each (the others share theirs out).
+    (64, 130, 16, 16, 32, True), (64, 200, 32, 16, 64, False), (32, 129, 16, 16, 128, True)])
 def test_shapes(B, S, H, Hkv, E, causal, dtype):
     check_all(*draw(B, S, H, Hkv, E, dtype, seed=S), causal)
 
