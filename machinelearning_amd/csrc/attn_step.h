@@ -29,6 +29,7 @@ struct StepParams {
   int nsplit;                          // key splits of a unit (16-bit: workgroups in all)
   int min_blocks;                      // 16-bit: key blocks that a workgroup takes at least
   float resc_th;                       // 16-bit: lazy-rescale threshold in raw score units
+  FastDiv div_rep, div_ups, div_ngrp;  // by rep; 16-bit: units per sequence, row groups
 };
 
 constexpr int kTreeMax = 256;          // nodes of a tree: one per thread of a workgroup

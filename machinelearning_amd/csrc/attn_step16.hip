@@ -28,6 +28,9 @@ namespace mi {
 
 namespace {
 
+template <int I>
+using ic = std::integral_constant<int, I>;
+
 template <int D, int MAPS, int NR, int NK>
 struct Step16 {
   static constexpr int MW = NR == 1 ? MAPS : 1;  // maps of a wave
@@ -54,53 +57,72 @@ struct Line {
   int N, per;
 };
 
-// A value that is the same in every lane, in a scalar register.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Sum over the lanes up to and including each (DPP: six VALU instructions).
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  add(ic<0x111>{}, ic<0xF>{});    // row_shr 1, 2, 4, 8: within rows of 16 lanes
+  add(ic<0x112>{}, ic<0xF>{});
+  add(ic<0x114>{}, ic<0xF>{});
+  add(ic<0x118>{}, ic<0xF>{});
+  add(ic<0x142>{}, ic<0xA>{});    // row_bcast15: a row's last lane to the odd rows behind it
+  add(ic<0x143>{}, ic<0xC>{});    // row_bcast31: lane 31 to the upper half
+  return x;
+}
+__device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 
-// Blocks of a unit of sequence b, the empty ones included.
+// The line as a wave sees it, 64 sequences at a time; the first 64 are kept in the lanes.
+struct Scan {
+  int len;            // cached rows of sequence `lane`
+  int own, upto;      // blocks of one of its units; of all sequences up to it
+};
+
 template <int SETUP>
-__device__ __forceinline__ int step_blocks(const StepParams& p, int b) {
-  return (step_len(p, b) + 31) / 32 + (p.T + 31) / 32 + SETUP;
+__device__ __forceinline__ Scan scan64(const StepParams& p, int b0) {
+  const int i = b0 + (int)(threadIdx.x & 63);
+  Scan s;
+  s.len = i < p.B ? step_len(p, i) : 0;
+  s.own = i < p.B ? (s.len + 31) / 32 + (p.T + 31) / 32 + SETUP : 0;
+  s.upto = wave_scan(s.own);
+  return s;
 }
 
-// Blocks of one unit of each sequence before `b`, all lanes of a wave.
 template <int SETUP>
-__device__ __forceinline__ int blocks_before(const StepParams& p, int b) {
-  int sum = 0;
-  for (int i = threadIdx.x & 63; i < b; i += 64) sum += step_blocks<SETUP>(p, i);
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-  return uniform(sum);
-}
-
-template <int SETUP>
-__device__ __forceinline__ Line step_line(const StepParams& p, int units_per_seq) {
-  const int N = blocks_before<SETUP>(p, p.B) * units_per_seq;
+__device__ __forceinline__ Line step_line(const StepParams& p, int units_per_seq, Scan& first) {
+  first = scan64<SETUP>(p, 0);
+  int N = lane_value(first.upto, 63);
+  for (int b0 = 64; b0 < p.B; b0 += 64) N += lane_value(scan64<SETUP>(p, b0).upto, 63);
+  N *= units_per_seq;
   return {N, max((int)(((unsigned)N + p.nsplit - 1) / (unsigned)p.nsplit), p.min_blocks)};
 }
 
-// The sequence that holds block x of one unit of each sequence, and the blocks before it:
-// a wave's scan, 64 sequences a round.
+// The sequence that holds block x of one unit of each sequence, and the blocks before it.
+// `s` becomes the scan that holds it.
 template <int SETUP>
-__device__ __forceinline__ int find_seq(const StepParams& p, int x, int& before) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ int find_seq(const StepParams& p, Scan& s, int x, int& before) {
   before = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int own = b0 + lane < p.B ? step_blocks<SETUP>(p, b0 + lane) : 0;
-    int upto = own;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int y = __shfl_up(upto, s);
-      if (lane >= s) upto += y;
-    }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + upto > x);
+    if (b0) s = scan64<SETUP>(p, b0);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + s.upto > x);
     if (past || b0 + 64 >= p.B) {
       const int l = past ? __builtin_ctzll(past) : min(63, p.B - 1 - b0);
-      before += uniform(__shfl(upto - own, l));
+      before += lane_value(s.upto, l) - lane_value(s.own, l);
       return b0 + l;
     }
-    before += uniform(__shfl(upto, 63));
+    before += lane_value(s.upto, 63);
   }
+}
+
+// Blocks of one unit of each sequence before `b`; `s` becomes the scan that holds b.
+template <int SETUP>
+__device__ __forceinline__ int blocks_before(const StepParams& p, Scan& s, int b) {
+  int sum = 0;
+  for (int b0 = 0; b0 + 64 <= b; b0 += 64) {
+    sum += lane_value(s.upto, 63);
+    s = scan64<SETUP>(p, b0 + 64);
+  }
+  return sum + lane_value(s.upto, b & 63) - lane_value(s.own, b & 63);
 }
 
 // A tree of at most 64 nodes in a wave's registers: lane t holds node t's line of descent
@@ -135,7 +157,7 @@ __device__ __forceinline__ void step16_emit(const StepParams& p, T* __restrict__
                                             int b, int kvh, int r, int d0, const f32x4 (&o)[MAPS],
                                             const float (&M)[MAPS], const float (&L)[MAPS], bool dead,
                                             bool poisoned) {
-  const int t = r / p.rep, h = kvh * p.rep + r % p.rep;
+  const int t = (int)fdiv((unsigned)r, p.div_rep), h = kvh * p.rep + r - t * p.rep;
   f32x4 y = o[0] * (1.f / L[0]);
   if constexpr (MAPS == 2) y -= o[1] * (load_as_float(p.lam, p.lam_dtype, h) / L[1]);
   if (p.gate) y *= 1.f / (1.f + __expf(-p.gate[((long long)b * p.T + t) * p.H + h]));
@@ -168,7 +190,10 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   const int l32 = lane & 31, g = lane >> 5;
   const int rw = wave % NR, mw = wave / NR % NM, kw = wave / NG;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;   // units per sequence
-  const Line line = step_line<C::SETUP>(p, ups);
+  // The arguments that are needed only behind the lengths: fetched beside them.
+  asm volatile("" ::"s"(Q), "s"(Vn), "s"(part), "s"(p.k_sb), "s"(p.v_sh), "s"(p.parents), "s"(p.div_ngrp.m));
+  Scan scan;
+  const Line line = step_line<C::SETUP>(p, ups, scan);
   // (Pieces past the line's end: none of the products passes 31 bits, nsplit and per being
   // chosen for the largest N.)
   const long long begin = (long long)blockIdx.x * line.per;
@@ -194,14 +219,14 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   const bool small_tree = TREE && p.T <= 64;
 
   int before;                             // blocks of one unit of each earlier sequence
-  int b = find_seq<C::SETUP>(p, at / ups, before);
+  int b = find_seq<C::SETUP>(p, scan, (int)fdiv((unsigned)at, p.div_ups), before);
   while (true) {
     // The fragment of unit u of sequence b that begins at `at`: its blocks [blk0, blk1).
-    const int Lc = step_len(p, b), ncb = (Lc + 31) / 32, nb = ncb + (p.T + 31) / 32;
+    const int Lc = lane_value(scan.len, b & 63), ncb = (Lc + 31) / 32, nb = ncb + (p.T + 31) / 32;
     const int span = nb + C::SETUP, in_seq = at - before * ups;
     const int u = in_seq / span, from = in_seq - u * span, to = min(span, from + end - at);
     const int blk0 = max(from - C::SETUP, 0), blk1 = to - C::SETUP;
-    const int kvh = u / ngrp, grp = u % ngrp;
+    const int kvh = (int)fdiv((unsigned)u, p.div_ngrp), grp = u - kvh * ngrp;
     const bool whole = blk0 == 0 && blk1 == nb, has_tail = blk1 > ncb;
     if (blk1 > blk0) {
 
@@ -239,9 +264,9 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
     // The wave's rows, in flight with the first blocks.
     const int r = (grp * NR + rw) * 32 + l32;
     const bool row = r < p.R;
-    const int t = row ? r / p.rep : 0;
+    const int t = row ? (int)fdiv((unsigned)r, p.div_rep) : 0;
     frag qf[DS];
-    const T* qrow = Q + (((long long)b * p.T + t) * p.H + kvh * p.rep + (row ? r % p.rep : 0)) * D;
+    const T* qrow = Q + (((long long)b * p.T + t) * p.H + kvh * p.rep + (row ? r - t * p.rep : 0)) * D;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qf[ds] = row ? ld_frag<T>(qrow + (mw * DS + ds) * 16 + g * 8) : zero_frag<T>();
     WaveTree wt = {0u, 0u, -1};
@@ -468,7 +493,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
     if (at >= end) break;
     if (u + 1 == ups) {                    // the sequence's last unit is done
       before += span;
-      ++b;
+      if ((++b & 63) == 0) scan = scan64<C::SETUP>(p, b);
     }
   }
 }
@@ -485,9 +510,10 @@ step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* 
   const int r = (int)(gr % p.R), kvh = (int)(gr / p.R % p.Hkv), b = (int)(gr / p.R / p.Hkv);
   const int lane = threadIdx.x & 63, q = lane % NQ, fg = lane / NQ;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS, ups = p.Hkv * ngrp;
-  const Line line = step_line<C::SETUP>(p, ups);
-  const int span = step_blocks<C::SETUP>(p, b), grp = r / C::ROWS, rr = r % C::ROWS;
-  const int start = blocks_before<C::SETUP>(p, b) * ups + (kvh * ngrp + grp) * span;
+  Scan scan;
+  const Line line = step_line<C::SETUP>(p, ups, scan);
+  const int grp = r / C::ROWS, rr = r % C::ROWS, before = blocks_before<C::SETUP>(p, scan, b);
+  const int span = lane_value(scan.own, b & 63), start = before * ups + (kvh * ngrp + grp) * span;
   const int g0 = (start + C::SETUP) / line.per, g1 = (start + span - 1) / line.per;
   if (g0 == g1) return;                            // written by the workgroup that had it all
   const float c = p.scale_log2;
@@ -548,6 +574,8 @@ void step16_geometry(StepParams& p) {
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS;
   const long long most = (long long)p.B * p.Hkv * ngrp * ((p.rows + 31) / 32 + (p.T + 31) / 32 + C::SETUP);
   p.min_blocks = 4 * NK;
+  p.div_ups = fast_div((unsigned)(p.Hkv * ngrp));
+  p.div_ngrp = fast_div((unsigned)ngrp);
   const long long want = (most + p.min_blocks - 1) / p.min_blocks;
   p.nsplit = (int)(want < 256 * per_cu ? want : 256 * per_cu);
 }
@@ -568,9 +596,6 @@ hipError_t step16_t(const void* q, const void* kc, const void* vc, const void* k
                      0, st, ws, (T*)out, lse, p);
   return hipGetLastError();
 }
-
-template <int I>
-using ic = std::integral_constant<int, I>;
 
 // f(D, MAPS, NR, NK) for a step: row waves by the row tiles of a kv head.
 template <typename F>

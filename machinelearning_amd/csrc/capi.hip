@@ -921,6 +921,7 @@ mi::StepParams step_params(const mi_step_shape* s) {
   p.lam_dtype = s->lam_dtype;
   p.R = s->T * p.rep;
   p.resc_th = 8.f / p.scale_log2;
+  p.div_rep = mi::fast_div((unsigned)p.rep);
   return p;
 }
 

@@ -297,6 +297,17 @@ def test_long_caches(B, T, H, Hkv, D, longest, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("B", [63, 64, 65, 128, 200])
+def test_many_sequences(B):
+    """The prefix sum over the lengths, 64 sequences a round."""
+    g = torch.Generator().manual_seed(B)
+    for T, H in ((1, 4), (5, 16)):
+        lens = torch.randint(0, 150, (B,), generator=g).to(torch.int32)
+        q, k, v, ck, cv, lam = draw(B, T, H, 2, 32, 150, torch.bfloat16, seed=T)
+        run(q, k, v, ck, cv, lens, draft(B, T, B, pad=True), lam if T > 1 else None)
+
+
+@gpu
 @pytest.mark.parametrize("shape", ["chain", "star", "roots"])
 @pytest.mark.parametrize("T", [31, 64, 130, 256])
 def test_tree_shapes(shape, T):
