@@ -63,7 +63,7 @@ enum { kDelta1 = 0, kSeed1 = 1, kSeed2 = 2, kCross = 3, kPlanes = 4 };
 // Forward: 64 query rows of one (batch, head) per workgroup.
 // ---------------------------------------------------------------------------
 template <typename T, int E>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(E <= 64 ? 3 : 2, 8)))
 diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                   T* __restrict__ O, T* __restrict__ O2, float* __restrict__ LSE, DiffParams p) {
   using C = Diff16<E>;
@@ -73,7 +73,8 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
   // Ring slot s: K tile ring[s][0], V tile ring[s][1]; unit u = {K tile u + 1, V tile u}.
   __shared__ __attribute__((aligned(1024))) char ring[NS][2][C::TILE];
   __shared__ __attribute__((aligned(1024))) char qstage[C::TILE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, g = lane >> 5;
   const int rw = wave & 1, mw = wave >> 1;         // row tile, map
   const WorkItem wi = work_item(p.nblk, p.B * p.H, p.div_wi, p.causal, p.wi_blocks_fastest);
@@ -102,10 +103,10 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
     for (int j = 0; j < C::LPW; ++j) dma16_buf(rq, qoff[j], m0q + (unsigned)(4096 * j));
   }
 
-  const int t_end = ((p.causal ? min(p.S, q0 + BM) : p.S) + BN - 1) / BN;
-  int tw_end = t_end;
-  if (qw0 >= p.S) tw_end = 0;
-  if (p.causal) tw_end = min(tw_end, (qw0 + 31) / BN + 1);
+  // The workgroup's rows end in the same key tile, so that its waves walk the same tiles and
+  // only the last one needs a mask.
+  static_assert(BM == BN, "one diagonal tile");
+  const int t_last = ((p.causal ? min(p.S, q0 + BM) : p.S) + BN - 1) / BN - 1;
 
   int kaddr[DH];
 #pragma unroll
@@ -120,24 +121,25 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
   float m_run = -1e30f, l_run = 0.f;
   const float c = p.scale_log2;
   const int key_hi = p.causal ? min(qi, p.S - 1) : p.S - 1;
-  const int wave_key_hi = p.causal ? qw0 : p.S;
+  const int wave_key_lo = p.causal ? qw0 : p.S - 1, wave_key_hi = min(p.causal ? qw0 + 31 : p.S, p.S - 1);
 
-  auto step = [&](auto slot_fill_c, auto par_c, int t) __attribute__((always_inline)) {
+  // One key tile, of which the first HALVES x 32 keys count. LAST: the masked one, which no
+  // other follows.
+  auto step = [&](auto slot_fill_c, auto par_c, auto last_c, auto halves_c, int t) __attribute__((always_inline)) {
     constexpr int SF = decltype(slot_fill_c)::value, SR = (SF + 1) % NS, PAR = decltype(par_c)::value;
-    wait_ring<LPU>(min(NS - 2, t_end - 1 - t));
-    lds_barrier();
-    if (t + NS - 1 <= t_end - 1) issue_unit(SF, t + NS - 1);
+    constexpr bool LAST = decltype(last_c)::value != 0;
+    constexpr int HALVES = decltype(halves_c)::value;
     const char* sK = ring[SR][0];
     const char* sV = ring[SR][1];
-    const bool cur = t < tw_end, nxt = t + 1 < tw_end;
     f32x16 (&s)[2] = sS[PAR];
-    if (!cur) return;
-    const int k0 = t * BN;
-    if (k0 + BN > p.S || (p.causal && k0 + BN - 1 > wave_key_hi)) {
+    if constexpr (LAST) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) mask_above(s[mt], key_hi - (k0 + mt * 32 + 4 * g), -INFINITY);
+      for (int mt = 0; mt < HALVES; ++mt) {
+        const int kb = t * BN + mt * 32;
+        if (kb + 31 > wave_key_lo) mask_above(s[mt], key_hi - (kb + 4 * g), -INFINITY);
+      }
     }
-    const float mx = max32(s[0], s[1]);
+    const float mx = HALVES == 2 ? max32(s[0], s[1]) : max32(s[0], s[0]);
     if (t == 0) {
       m_run = fmaxf(m_run, halves_max(mx));
     } else if (wave_any(mx > m_run + p.resc_th)) {
@@ -158,9 +160,12 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
       if (idx < 4) rs[idx] = s[mt][r];
       else rs[idx & 3] += s[mt][r];
     };
-    // The next tile's score MFMAs, each followed by a slice of this tile's exps.
-    constexpr int NM = 2 * DH, EPM = 32 / NM, LAK = 2;
-    if (nxt) {
+    if constexpr (LAST) {
+#pragma unroll
+      for (int i = 0; i < 16 * HALVES; ++i) prob(i);
+    } else {
+      // The next tile's score MFMAs, each followed by a slice of this tile's exps.
+      constexpr int NM = 2 * DH, EPM = 32 / NM, LAK = 2;
       f32x16 (&sn)[2] = sS[PAR ^ 1];
       frag kfr[NM];
       auto kread = [&](int i) __attribute__((always_inline)) {
@@ -178,13 +183,10 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
         for (int e = 0; e < EPM; ++e) prob(i * EPM + e);
         __builtin_amdgcn_sched_barrier(0);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) prob(i);
     }
     l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     // O^T += V^T P^T, V^T fragments LAV MFMAs ahead.
-    constexpr int NP = 4 * DT, LAV = E >= 128 ? 2 : 1;
+    constexpr int NP = 2 * HALVES * DT, LAV = E >= 128 ? 2 : 1;
     auto vread = [&](int j) __attribute__((always_inline)) {
       const int mt = j / (2 * DT), ks = (j / DT) & 1, dt = j % DT;
       const int roff = (32 * mt + 16 * ks) * E * 2;
@@ -205,25 +207,40 @@ diff16_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __r
 
 #pragma unroll
   for (int i = 0; i < NS; ++i)
-    if (i - 1 <= t_end - 1) issue_unit(i, i - 1);
+    if (i - 1 <= t_last) issue_unit(i, i - 1);
   __builtin_amdgcn_s_waitcnt(kWaitVm0);
   lds_barrier();
 #pragma unroll
   for (int ds = 0; ds < DH; ++ds)
     qf[ds] = lds_frag<T>(qstage + tile_off<E>(32 * rw + l32, 2 * (mw * DH + ds) + g));
-  if (tw_end > 0) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      sS[0][mt] = zero16();
+  for (int mt = 0; mt < 2; ++mt) {
+    sS[0][mt] = zero16();
 #pragma unroll
-      for (int ds = 0; ds < DH; ++ds)
-        sS[0][mt] = M::mma(lds_frag<T>(ring[0][0] + kaddr[ds] + mt * 32 * E * 2), qf[ds], sS[0][mt]);
+    for (int ds = 0; ds < DH; ++ds)
+      sS[0][mt] = M::mma(lds_frag<T>(ring[0][0] + kaddr[ds] + mt * 32 * E * 2), qf[ds], sS[0][mt]);
+  }
+  // (All that the ring will ever hold has been asked for: nothing to wait for behind it.)
+  auto fill = [&](auto slot_c, int t) __attribute__((always_inline)) {
+    wait_ring<LPU>(min(NS - 2, t_last - t));
+    lds_barrier();
+    if (t + NS - 1 <= t_last) issue_unit(decltype(slot_c)::value, t + NS - 1);
+  };
+  auto last = [&](auto par_c) __attribute__((always_inline)) {
+    fill(par_c, t_last);
+    if (t_last * BN + 32 > wave_key_hi) step(par_c, par_c, ic<1>{}, ic<1>{}, t_last);
+    else step(par_c, par_c, ic<1>{}, ic<2>{}, t_last);
+  };
+  for (int t = 0; t < t_last; t += 2) {
+    fill(ic<0>{}, t);
+    step(ic<0>{}, ic<0>{}, ic<0>{}, ic<2>{}, t);
+    if (t + 1 < t_last) {
+      fill(ic<1>{}, t + 1);
+      step(ic<1>{}, ic<1>{}, ic<0>{}, ic<2>{}, t + 1);
     }
   }
-  for (int t = 0; t < t_end; t += 2) {
-    step(ic<0>{}, ic<0>{}, t);
-    if (t + 1 < t_end) step(ic<1>{}, ic<1>{}, t + 1);
-  }
+  if (t_last & 1) last(ic<1>{});
+  else last(ic<0>{});
 
   // The second map's rows, normalised, to the first map's wave: quad after quad, a lane's
   // own 16 bytes each.
