@@ -10,6 +10,7 @@
 //    map's dS feeds its own half of dQ.
 //  * dK/dV: a wave owns 32 keys of both maps: dV takes (P_1 - lam P_2)^T dO in one product.
 #include <type_traits>
+#include <utility>
 
 #include "attn16.h"
 #include "attn_diff.h"
@@ -20,6 +21,16 @@ namespace {
 
 template <int I>
 using ic = std::integral_constant<int, I>;
+
+// f(ic<0>), ..., f(ic<N - 1>): a loop whose counter is a constant in its body.
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(ic<I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
 
 template <int N>
 __device__ __forceinline__ void wait_ring(int n) {
@@ -519,8 +530,8 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
   using C = Diff16<E>;
   using M = Mfma32<T>;
   using frag = typename M::frag;
-  constexpr int BK = 128, BQ = C::BN, NS = 2, DS = C::DS, DH = C::DH, DT = C::DT;
-  constexpr int LPU = 2 * C::LPW + kPlanes;
+  constexpr int BK = 128, BQ = C::BN, NS = 4, DS = C::DS, DH = C::DH, DT = C::DT;
+  // Filled and drained two slots at a time: a barrier for 128 query rows.
   __shared__ __attribute__((aligned(1024))) char ring[NS][2][C::TILE];   // Q, dO
   __shared__ __attribute__((aligned(16))) float vecs[NS][kPlanes][BQ];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -564,12 +575,14 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
     u32x4 bits = __builtin_bit_cast(u32x4, vv);
     bits ^= 0x80008000u;                           // sign of every 16-bit element
     vf[ds] = __builtin_bit_cast(frag, bits);
+    if constexpr (E >= 128) {
+      // One wave per SIMD: 256 more registers, which MFMA reads its operands from.
+      asm("" : "+a"(kf[ds]));
+      asm("" : "+a"(vf[ds]));
+    }
   }
   const int tq_begin = p.causal ? k0 / BQ : 0, tq_end = (p.S + BQ - 1) / BQ;
   const int ntq = tq_end - tq_begin, niter = LINE ? f1 - f0 : p.group * ntq;
-  int tw_begin = tq_begin;
-  if (p.causal) tw_begin = kw0 / BQ;
-  if (kw0 >= p.S) tw_begin = tq_end;
 
   unsigned dvoff[C::LPW];
   dma_offsets<E>(dvoff, wave, lane, p.q_rs);
@@ -620,103 +633,162 @@ diff16_dkdv_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __
   const float c = p.scale_log2;
   const int q_lo = p.causal ? kj : 0, wave_q_lo = p.causal ? kw0 + 31 : 0;
 
-  auto seed = [&](const float* v, int mt) __attribute__((always_inline)) {
-    f32x16 a;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 v4 = *reinterpret_cast<const f32x4*>(v + mt * 32 + 8 * j + 4 * g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[4 * j + e] = v4[e];
-    }
-    return a;
+  // The MFMAs of 32 query rows in their order: S_1 and S_2 in turn, G, then for each 16 rows
+  // dV and dK. Each one's LDS operand is read LA of them ahead, over the ends of halves and
+  // tiles (of a pair) too, as the accumulators' seeds are.
+  constexpr int PK = C::SHARED ? 3 : 2 * DT, NM = 2 * DS + 2 * PK, LA = E >= 128 ? 4 : 2;
+  int vaddr = 4 * g;                               // floats into vecs
+  auto operand = [&](int u, int mt, int i) __attribute__((always_inline)) {
+    const char* sQ = &ring[0][0][0] + u * 2 * C::TILE + mt * 32 * E * 2;
+    const char* sO = sQ + C::TILE;
+    if (i < DS) return lds_frag<T>(sQ + qaddr[(i & 1) * DH + (i >> 1)]);
+    if (i < 2 * DS) return lds_frag<T>(sO + qaddr[i - DS]);
+    const int ks = (i - 2 * DS) / PK, x = (i - 2 * DS) % PK, dt = C::SHARED ? 0 : x >> 1;
+    const char* t = (x & 1 ? sQ : sO) + 16 * ks * E * 2;
+    return lds_frag_tr<T>(t + ttoff[dt][0], t + ttoff[dt][1]);
   };
-  // One query tile, in halves of 32 rows.
-  auto compute = [&](const char* sQ, const char* sO, const float (*sv)[BQ], int tq, float lam) __attribute__((always_inline)) {
+  // Elements 4j .. 4j + 3 of an accumulator's plane.
+  auto quad = [&](f32x16& a, int plane, int u, int mt, int j) __attribute__((always_inline)) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(&vecs[0][0][0] + vaddr + (u * kPlanes + plane) * BQ + mt * 32 + 8 * j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[4 * j + e] = v[e];
+  };
+  f32x16 s1, s2, ga;                               // seeds of the next 32 rows, and these
+  frag ahead[LA];
+  auto seed = [&](int u, int mt, int x) __attribute__((always_inline)) {
+    if (x < 4) quad(s1, kSeed1, u, mt, x);
+    else if (x < 8) quad(s2, kSeed2, u, mt, x - 4);
+    else quad(ga, kDelta1, u, mt, x - 8);
+  };
+  auto start = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 12; ++x) seed(u, 0, x);
+#pragma unroll
+    for (int i = 0; i < LA; ++i) ahead[i] = operand(u, 0, i);
+  };
+  // Query tile tq in slot u of the pair, in halves of 32 rows; `start` has been called for it.
+  auto compute = [&](auto u_c, int tq, float lam) __attribute__((always_inline)) {
+    constexpr int U = decltype(u_c)::value;
     const int q0 = tq * BQ;
     const bool need_lo = p.causal && q0 < wave_q_lo, need_hi = q0 + BQ > p.S;
+    each<2>([&](auto mt_c) __attribute__((always_inline)) {
+      constexpr int mt = decltype(mt_c)::value;
+      constexpr bool more = mt == 0 || U == 0;     // another half follows: its unit and half
+      constexpr int nu = mt == 0 ? U : 1, nmt = mt ^ 1;
+      frag fr[NM];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const int roff0 = mt * 32 * E * 2;
-      f32x16 s1 = seed(sv[kSeed1], mt), s2 = seed(sv[kSeed2], mt), ga = seed(sv[kDelta1], mt);
-      frag fr[DS];
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) fr[ds] = lds_frag<T>(sQ + qaddr[ds] + roff0);
-#pragma unroll
-      for (int ds = 0; ds < DH; ++ds) {
-        s1 = M::mma(fr[ds], kf[ds], s1);
-        s2 = M::mma(fr[DH + ds], kf[DH + ds], s2);
-      }
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) fr[ds] = lds_frag<T>(sO + qaddr[ds] + roff0);
-      constexpr int EPM = 16 / DS;
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) {
-        ga = M::mma(fr[ds], vf[ds], ga);
-#pragma unroll
-        for (int e = ds * EPM; e < (ds + 1) * EPM; ++e) {
-          s1[e] = fast_exp2(s1[e] * c);
-          s2[e] = fast_exp2(s2[e] * c);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (need_lo || need_hi) {
-        const int qb = q0 + mt * 32 + 4 * g;
-        unsigned keep = need_lo ? keep_from(q_lo - qb) : ~0u;
-        if (need_hi) keep &= keep_upto(p.S - 1 - qb);
-        mask_keep(s1, keep, 0.f);
-        mask_keep(s2, keep, 0.f);
-      }
-      const f32x16 cr = seed(sv[kCross], mt);
+      for (int i = 0; i < LA; ++i) fr[i] = ahead[i];
+      f32x16 cr, w;
       frag wf[2], f1[2], f2[2];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        f32x16 w;
-#pragma unroll
-        for (int e = ks * 8; e < ks * 8 + 8; ++e) {
-          w[e] = fmaf(-lam, s2[e], s1[e]);
-          s1[e] *= ga[e];
-          s2[e] *= fmaf(lam, ga[e], cr[e]);
-        }
+      auto elem = [&](int e) __attribute__((always_inline)) {
+        w[e] = fmaf(-lam, s2[e], s1[e]);
+        s1[e] *= ga[e];
+        s2[e] *= fmaf(lam, ga[e], cr[e]);
+      };
+      auto pack = [&](int ks) __attribute__((always_inline)) {
         wf[ks] = pack_frag<T>(w, ks * 8);
         f1[ks] = pack_frag<T>(s1, ks * 8);
         f2[ks] = pack_frag<T>(s2, ks * 8);
-      }
+      };
+      each<NM>([&](auto i_c) __attribute__((always_inline)) {
+        constexpr int i = decltype(i_c)::value;
+        constexpr int ks = i < 2 * DS ? -1 : (i - 2 * DS) / PK, x = i < 2 * DS ? 0 : (i - 2 * DS) % PK;
+        // This one's place in time: what is read for later ones.
+        if constexpr (i + LA < NM) {
+          constexpr bool again = C::SHARED && i + LA >= 2 * DS && (i + LA - 2 * DS) % PK == 2;
+          fr[i + LA] = again ? fr[i + LA - 1] : operand(U, mt, i + LA);
+        } else if constexpr (more) {
+          ahead[i + LA - NM] = operand(nu, nmt, i + LA - NM);
+        }
+        if constexpr (i == 2 * DS - 2) {
+          quad(cr, kCross, U, mt, 0);
+          quad(cr, kCross, U, mt, 1);
+        }
+        if constexpr (i == 2 * DS) {
+          quad(cr, kCross, U, mt, 2);
+          quad(cr, kCross, U, mt, 3);
+        }
+        if constexpr (ks == 1 && more) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+          for (int y = 12 * x / PK; y < 12 * (x + 1) / PK; ++y) seed(nu, nmt, y);
+        }
+        if constexpr (i == 2 * DS) {
+          if (need_lo || need_hi) {
+            const int qb = q0 + mt * 32 + 4 * g;
+            unsigned keep = need_lo ? keep_from(q_lo - qb) : ~0u;
+            if (need_hi) keep &= keep_upto(p.S - 1 - qb);
+            mask_keep(s1, keep, 0.f);
+            mask_keep(s2, keep, 0.f);
+          }
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const int roff = roff0 + 16 * ks * E * 2;
-          dv[dt] = M::mma(lds_frag_tr<T>(sO + ttoff[dt][0] + roff, sO + ttoff[dt][1] + roff), wf[ks], dv[dt]);
-          const frag qt = lds_frag_tr<T>(sQ + ttoff[dt][0] + roff, sQ + ttoff[dt][1] + roff);
-          if constexpr (C::SHARED) {
-            dk[0] = M::mma(qt, f1[ks], dk[0]);
-            dk[1] = M::mma(qt, f2[ks], dk[1]);
-          } else {
-            dk[dt] = M::mma(qt, dt < DT / 2 ? f1[ks] : f2[ks], dk[dt]);
+          for (int e = 0; e < 8; ++e) elem(e);
+          pack(0);
+        }
+        if constexpr (i < DS) {
+          if constexpr (i & 1) s2 = M::mma(fr[i], kf[DH + (i >> 1)], s2);
+          else s1 = M::mma(fr[i], kf[i >> 1], s1);
+        } else if constexpr (i < 2 * DS) {
+          ga = M::mma(fr[i], vf[i - DS], ga);
+          constexpr int EPM = 16 / DS;
+#pragma unroll
+          for (int e = (i - DS) * EPM; e < (i - DS + 1) * EPM; ++e) {
+            s1[e] = fast_exp2(s1[e] * c);
+            s2[e] = fast_exp2(s2[e] * c);
+          }
+        } else {
+          constexpr int dt = C::SHARED ? 0 : x >> 1;
+          if constexpr (x == 0 || (!C::SHARED && !(x & 1))) dv[dt] = M::mma(fr[i], wf[ks], dv[dt]);
+          else if constexpr (C::SHARED) dk[x - 1] = M::mma(fr[i], x == 1 ? f1[ks] : f2[ks], dk[x - 1]);
+          else dk[dt] = M::mma(fr[i], dt < DT / 2 ? f1[ks] : f2[ks], dk[dt]);
+          // The other 16 rows' factors under this 16 rows' MFMAs.
+          if constexpr (ks == 0) {
+#pragma unroll
+            for (int e = 8 + 8 * x / PK; e < 8 + 8 * (x + 1) / PK; ++e) elem(e);
+            if constexpr (x == PK - 1) pack(1);
           }
         }
-    }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
   };
 
-  float lam = load_as_float(p.lam, p.lam_dtype, cp_h);
-  auto step = [&](auto slot_c, int it) __attribute__((always_inline)) {
-    constexpr int SL = decltype(slot_c)::value;
-    wait_ring<LPU>(min(NS - 2, niter - 1 - it));
-    lds_barrier();
-    if (it + NS - 1 < niter) issue((SL + NS - 1) % NS);
-    if (cp_tq >= tw_begin) compute(ring[SL][0], ring[SL][1], vecs[SL], cp_tq, lam);
+  // (To a scalar at once: a load still open would be waited for where lam is used, and every
+  // DMA in flight with it.)
+  auto lam_of = [&](int h) __attribute__((always_inline)) {
+    const float x = load_as_float(p.lam, p.lam_dtype, h);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+  };
+  float lam = lam_of(cp_h);
+  auto advance = [&](int it) __attribute__((always_inline)) {
     if (++cp_tq == tq_end && it + 1 < niter) {
       cp_tq = tq_begin;
-      lam = load_as_float(p.lam, p.lam_dtype, ++cp_h);
+      lam = lam_of(++cp_h);
     }
   };
+  issue(0);
+  if (niter > 1) issue(1);
+  int turn = 1;                                    // which way the next pair of slots lies
+  for (int it = 0; it < niter; it += 2) {
+    wait_vm<0>();
+    lds_barrier();
+    if (it + 2 < niter) issue(turn > 0 ? 2 : 0);
+    if (it + 3 < niter) issue(turn > 0 ? 3 : 1);
+    start(0);
+    compute(ic<0>{}, cp_tq, lam);
+    advance(it);
+    if (it + 1 < niter) {
+      compute(ic<1>{}, cp_tq, lam);
+      advance(it + 1);
+    }
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < niter) issue(i);
-  __builtin_amdgcn_s_waitcnt(kWaitVm0);
-  for (int it = 0; it < niter; it += NS) {
-    step(ic<0>{}, it);
-    if (it + 1 < niter) step(ic<1>{}, it + 1);
+    for (int ds = 0; ds < DS; ++ds) qaddr[ds] += turn * 4 * C::TILE;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      ttoff[dt][0] += turn * 4 * C::TILE;
+      ttoff[dt][1] += turn * 4 * C::TILE;
+    }
+    vaddr += turn * 2 * kPlanes * BQ;
+    turn = -turn;
   }
 
   lds_barrier();
