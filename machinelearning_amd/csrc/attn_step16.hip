@@ -11,11 +11,13 @@
 //    a unit that one fragment covers is written at once, the others' fragments go to the
 //    workspace as float32 partials (at most the first and the last of a piece are partial:
 //    two slots per workgroup) and step16_combine_kernel merges them in order.
+//    A cache of few rows takes none of this: a workgroup per unit (kDirectSteps).
 //  * Waves. NR row waves x NM map waves x NK key groups. Up to 32 rows, each of four waves
 //    takes every fourth block (its own LDS ring, no barrier in the loop) and both maps;
 //    with more rows, a group's waves share the blocks of its ring, a row tile and a map
-//    each (two 128-wide maps' sums of 32 rows would fill half of the registers). A wave's scores are transposed, S^T = K Q^T, so a lane owns a
-//    query row and P^T feeds O^T += V^T P^T from registers (attn16.h's tiles).
+//    each (two 128-wide maps' sums of 32 rows would fill half of the registers). A wave's
+//    scores are transposed, S^T = K Q^T, so a lane owns a query row and P^T feeds
+//    O^T += V^T P^T from registers (attn16.h's tiles).
 //  * Masks only where a block needs one: a sequence's last cached block (rows past it read
 //    as zeros through the buffer's bound) and the active block's, one word per block.
 #include <type_traits>
@@ -193,13 +195,25 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   // The arguments that are needed only behind the lengths: fetched beside them.
   asm volatile("" ::"s"(Q), "s"(Vn), "s"(part), "s"(p.k_sb), "s"(p.v_sh), "s"(p.parents), "s"(p.div_ngrp.m));
   Scan scan;
-  const Line line = step_line<C::SETUP>(p, ups, scan);
-  // (Pieces past the line's end: none of the products passes 31 bits, nsplit and per being
-  // chosen for the largest N.)
-  const long long begin = (long long)blockIdx.x * line.per;
-  if (begin >= line.N) return;
-  int at = (int)begin;
-  const int end = line.N - at > line.per ? at + line.per : line.N;
+  Line line = {0, 0};
+  int at = 0, end = 0, b = 0, before = 0;   // this piece of the line; blocks of one unit of each earlier sequence
+  if (p.direct) {
+    b = (int)fdiv(blockIdx.x, p.div_ups);
+    scan.len = step_len(p, b);
+    scan.own = (scan.len + 31) / 32 + (p.T + 31) / 32 + C::SETUP;
+    at = ((int)blockIdx.x - b * ups) * scan.own;
+    end = at + scan.own;
+  } else {
+    line = step_line<C::SETUP>(p, ups, scan);
+    // (Pieces past the line's end: none of the products passes 31 bits, nsplit and per being
+    // chosen for the largest N.)
+    const long long first = (long long)blockIdx.x * line.per;
+    if (first >= line.N) return;
+    at = (int)first;
+    end = line.N - at > line.per ? at + line.per : line.N;
+    b = find_seq<C::SETUP>(p, scan, (int)fdiv((unsigned)at, p.div_ups), before);
+  }
+  const int begin = at;
 
   char* ring = lds + kw * (NS * 2 * TILE);
   int kaddr[DS];
@@ -218,8 +232,6 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
   const float c = p.scale_log2;
   const bool small_tree = TREE && p.T <= 64;
 
-  int before;                             // blocks of one unit of each earlier sequence
-  int b = find_seq<C::SETUP>(p, scan, (int)fdiv((unsigned)at, p.div_ups), before);
   while (true) {
     // The fragment of unit u of sequence b that begins at `at`: its blocks [blk0, blk1).
     const int Lc = lane_value(scan.len, b & 63), ncb = (Lc + 31) / 32, nb = ncb + (p.T + 31) / 32;
@@ -398,7 +410,7 @@ step16_kernel(const T* __restrict__ Q, const T* __restrict__ Kc, const T* __rest
     }
 
     // The fragment's result. l < 0 marks a row outside the tree, m = NaN a poisoned one.
-    const int slot = 2 * blockIdx.x + (at != (int)begin);
+    const int slot = 2 * blockIdx.x + (at != begin);
     float* po = part + (long long)slot * C::SLOT;
     float* pml = po + C::ROWS * MAPS * D;
 #pragma unroll
@@ -565,6 +577,14 @@ step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* 
 
 namespace {
 
+// Steps (NK blocks each) up to which a workgroup takes a whole unit by itself. Against the
+// line, us a call: 16 sequences x 12 kv heads of D = 64, two maps, one token, 300 / 1000 /
+// 1500 cached rows (3, 9, 12 steps) 8.4 / 15.3 / 18.8 against 13.8 / 18.9 / 22.7; 32 x 8 of
+// D = 128, lengths drawn from 0 to 300 / 1000 / 2000: 12.5 / 23.5 / 38.8 against 18.1 / 26.3 /
+// 39.5; but 20 x 8 of lengths up to 2000 (16 steps) 31.0 against 28.1, and one sequence of two
+// kv heads 7.5 / 11.9 / 14.1 (300 / 1000 / 1500 rows) against 11.2 / 11.0 / 12.2.
+constexpr int kDirectSteps = 10;
+
 // Workgroups of a launch: what the chip holds at once (by LDS and registers), fewer where
 // the longest batch that the cache can hold has less than min_blocks for each.
 template <int D, int MAPS, int NR, int NK>
@@ -578,6 +598,10 @@ void step16_geometry(StepParams& p) {
   p.div_ngrp = fast_div((unsigned)ngrp);
   const long long want = (most + p.min_blocks - 1) / p.min_blocks;
   p.nsplit = (int)(want < 256 * per_cu ? want : 256 * per_cu);
+  // Short caches: a workgroup per unit, with no line to find a place in, no partials and no
+  // second launch.
+  p.direct = ((p.rows + 31) / 32 + (p.T + 31) / 32 + NK - 1) / NK <= kDirectSteps;
+  if (p.direct) p.nsplit = (int)((long long)p.B * p.Hkv * ngrp);
 }
 
 template <typename T, int D, int MAPS, int NR, int NK>
@@ -591,6 +615,7 @@ hipError_t step16_t(const void* q, const void* kc, const void* vc, const void* k
   };
   if (p.parents) go(std::true_type{});
   else go(std::false_type{});
+  if (p.direct) return hipGetLastError();
   const long long rows = (long long)p.B * p.Hkv * p.R;
   hipLaunchKernelGGL((step16_combine_kernel<T, D, MAPS, NR, NK>), dim3((unsigned)((rows + 3) / 4)), dim3(256),
                      0, st, ws, (T*)out, lse, p);
@@ -620,7 +645,7 @@ long long step16_workspace_floats(const StepParams& p, int D, bool two_maps) {
     using C = Step16<decltype(d)::value, decltype(m)::value, decltype(nr)::value, decltype(nk)::value>;
     StepParams g = p;
     step16_geometry<decltype(d)::value, decltype(m)::value, decltype(nr)::value, decltype(nk)::value>(g);
-    return 2LL * g.nsplit * C::SLOT;
+    return g.direct ? 0LL : 2LL * g.nsplit * C::SLOT;
   });
 }
 

@@ -22,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -245,17 +246,22 @@ struct Diff : torch::autograd::Function<Diff> {
     return s;
   }
 
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
-                        const Tensor& lam, int64_t causal, double scale, bool keep) {
-    const c10::DeviceGuard guard(q.device());
+  static Tensor run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, int64_t causal,
+                    double scale, const Tensor& o2, const Tensor& lse) {
     const mi_diff_shape s = shape(q, k, lam, causal, scale);
-    Tensor out = at::empty_like(q), o2, lse;
-    if (keep) {   // what the backward reads
-      o2 = at::empty_like(q);
-      lse = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    }
+    Tensor out = at::empty_like(q);
     check(mi_attn_diff_fwd(ptr(q), ptr(k), ptr(v), ptr(lam), ptr(out), ptr(o2), floats(lse), &s,
                            stream_of(q)));
+    return out;
+  }
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Tensor& lam, int64_t causal, double scale) {
+    const c10::DeviceGuard guard(q.device());
+    // What the backward reads.
+    const Tensor o2 = at::empty_like(q);
+    const Tensor lse = at::empty({2, q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    Tensor out = run(q, k, v, lam, causal, scale, o2, lse);
     ctx->save_for_backward({q, k, v, lam, out, o2, lse});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
@@ -284,7 +290,7 @@ struct Diff : torch::autograd::Function<Diff> {
       out = {dq, dk, dv, dlam};
     }
     out = once(grads, std::move(out));
-    out.resize(7);
+    out.resize(6);
     return out;
   }
 };
@@ -372,12 +378,20 @@ PyObject* py_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t causal = PyLong_AsLongLong(args[4]);
   const double scale = PyFloat_AsDouble(args[5]);
   if (PyErr_Occurred()) throw python_error();
-  const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
-                                                   v.requires_grad() || lam.requires_grad());
+  // A node only where one is needed (a forward-mode tangent is the node's to refuse).
+  bool node = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
+                                             v.requires_grad() || lam.requires_grad());
+  for (const Tensor* t : {&q, &k, &v, &lam}) node = node || torch::autograd::isFwGradDefined(*t);
   Tensor out;
   {
     pybind11::gil_scoped_release no_gil;
-    out = Diff::apply(q, k, v, lam, causal, scale, keep);
+    if (node) {
+      out = Diff::apply(q, k, v, lam, causal, scale);
+    } else {
+      at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(q.device());
+      out = Diff::run(q, k, v, lam, causal, scale, Tensor(), Tensor());
+    }
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

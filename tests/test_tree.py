@@ -140,7 +140,7 @@ def test_abi_refuses_shapes(kw, code):
 
 
 def test_abi_refuses_pointers():
-    lib, s = _capi.load(), step_shape()
+    lib, s = _capi.load(), step_shape(rows=5000)     # enough for a workspace
     good = [0x1000] * 5 + [0x1004, 0x1004, None, None, 0x1000, None, 0x1000]
 
     def step(**kw):
@@ -151,7 +151,7 @@ def test_abi_refuses_pointers():
     for i in (0, 1, 2, 3, 4, 9, 11):
         assert step(**{f"a{i}": None}) == 1, i
         assert step(**{f"a{i}": 0x1008}) == 6, i
-    two = step_shape(maps=2)
+    two = step_shape(maps=2, rows=5000)
     assert lib.mi_attn_step(*good, ctypes.byref(two), None) == 1          # no lam
     with_lse = list(good)
     with_lse[7], with_lse[10] = 0x1000, 0x1000
@@ -305,6 +305,23 @@ def test_many_sequences(B):
         lens = torch.randint(0, 150, (B,), generator=g).to(torch.int32)
         q, k, v, ck, cv, lam = draw(B, T, H, 2, 32, 150, torch.bfloat16, seed=T)
         run(q, k, v, ck, cv, lens, draft(B, T, B, pad=True), lam if T > 1 else None)
+
+
+@gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", DT, ids=name)
+def test_room_to_spare(D, dtype):
+    """Short sequences in a cache that could hold long ones: the steps' work is dealt out by
+    what it could hold (the tests of short caches run a workgroup for each unit)."""
+    for n, (B, T, rep, lens) in enumerate([
+            (4, 1, 1, [0, 1, 31, 32]), (4, 1, 4, [33, 1399, 100, 0]), (4, 16, 2, [0, 63, 65, 1]),
+            (4, 17, 3, [96, 7, 1400, 50]), (3, 33, 1, [31, 320, 0]), (2, 40, 8, [12, 777]),
+            (70, 3, 2, [11 * i % 150 for i in range(70)])]):
+        print((B, T, rep, lens), flush=True)
+        q, k, v, ck, cv, lam = draw(B, T, 2 * rep, 2, D, 1400, dtype, seed=n)
+        at = torch.tensor(lens, dtype=torch.int32)
+        for maps in (None, lam):
+            run(q, k, v, ck, cv, at, draft(B, T, n, pad=n % 2 == 1), maps)
 
 
 @gpu
