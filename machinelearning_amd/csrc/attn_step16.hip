@@ -11,7 +11,7 @@
 //    a unit that one fragment covers is written at once, the others' fragments go to the
 //    workspace as float32 partials (at most the first and the last of a piece are partial:
 //    two slots per workgroup) and step16_combine_kernel merges them in order.
-//    A cache of few rows takes none of this: a workgroup per unit (kDirectSteps).
+//    A cache of few rows takes none of this: a workgroup per unit (direct_steps).
 //  * Waves. NR row waves x NM map waves x NK key groups. Up to 32 rows, each of four waves
 //    takes every fourth block (its own LDS ring, no barrier in the loop) and both maps;
 //    with more rows, a group's waves share the blocks of its ring, a row tile and a map
@@ -577,13 +577,17 @@ step16_combine_kernel(const float* __restrict__ part, T* __restrict__ O, float* 
 
 namespace {
 
-// Steps (NK blocks each) up to which a workgroup takes a whole unit by itself. Against the
-// line, us a call: 16 sequences x 12 kv heads of D = 64, two maps, one token, 300 / 1000 /
-// 1500 cached rows (3, 9, 12 steps) 8.4 / 15.3 / 18.8 against 13.8 / 18.9 / 22.7; 32 x 8 of
-// D = 128, lengths drawn from 0 to 300 / 1000 / 2000: 12.5 / 23.5 / 38.8 against 18.1 / 26.3 /
-// 39.5; but 20 x 8 of lengths up to 2000 (16 steps) 31.0 against 28.1, and one sequence of two
-// kv heads 7.5 / 11.9 / 14.1 (300 / 1000 / 1500 rows) against 11.2 / 11.0 / 12.2.
-constexpr int kDirectSteps = 10;
+// Steps (NK blocks each) up to which a workgroup takes a whole unit by itself: ten where the
+// units are half the compute units or more, else what a lone workgroup's steps cost less than
+// the line's partials and second launch. Against the line, us a call: 16 sequences x 12 kv
+// heads of D = 64, two maps, one token, 300 / 1000 / 1500 rows (3, 9, 12 steps) 8.4 / 15.3 /
+// 18.8 for 13.8 / 18.9 / 22.7; 32 x 8 of D = 128, lengths drawn from 0 to 300 / 1000: 12.5 /
+// 23.5 for 18.1 / 26.3; but 20 x 8 of up to 2000 rows (16 steps) 31.0 for 28.1. Few units:
+// 24 x 2 of D = 128, 500 / 750 / 1000 rows (4, 6, 8 steps) 14.1 / 16.6 / 19.0 for 16.6 / 17.2
+// / 17.4; 6 x 2 of D = 64, 750 / 1000 / 1250 rows 10.8 / 12.5 / 13.6 for 12.3 / 12.5 / 12.1.
+__host__ constexpr int direct_steps(int D, long long units) {
+  return units >= 128 ? 10 : D >= 128 ? 6 : 8;
+}
 
 // Workgroups of a launch: what the chip holds at once (by LDS and registers), fewer where
 // the longest batch that the cache can hold has less than min_blocks for each.
@@ -600,8 +604,9 @@ void step16_geometry(StepParams& p) {
   p.nsplit = (int)(want < 256 * per_cu ? want : 256 * per_cu);
   // Short caches: a workgroup per unit, with no line to find a place in, no partials and no
   // second launch.
-  p.direct = ((p.rows + 31) / 32 + (p.T + 31) / 32 + NK - 1) / NK <= kDirectSteps;
-  if (p.direct) p.nsplit = (int)((long long)p.B * p.Hkv * ngrp);
+  const long long units = (long long)p.B * p.Hkv * ngrp;
+  p.direct = ((p.rows + 31) / 32 + (p.T + 31) / 32 + NK - 1) / NK <= direct_steps(D, units);
+  if (p.direct) p.nsplit = (int)units;
 }
 
 template <typename T, int D, int MAPS, int NR, int NK>

@@ -367,6 +367,19 @@ PyObject* py_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+Tensor diff_out(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, int64_t causal,
+                double scale) {
+  // A node only where one is needed (a forward-mode tangent is the node's to refuse).
+  bool node = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
+                                             v.requires_grad() || lam.requires_grad());
+  for (const Tensor* t : {&q, &k, &v, &lam}) node = node || torch::autograd::isFwGradDefined(*t);
+  pybind11::gil_scoped_release no_gil;
+  if (node) return Diff::apply(q, k, v, lam, causal, scale);
+  at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(q.device());
+  return Diff::run(q, k, v, lam, causal, scale, Tensor(), Tensor());
+}
+
 // diff_attn(q, k, v, lam, causal, scale) -> out.
 PyObject* py_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -378,28 +391,15 @@ PyObject* py_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t causal = PyLong_AsLongLong(args[4]);
   const double scale = PyFloat_AsDouble(args[5]);
   if (PyErr_Occurred()) throw python_error();
-  // A node only where one is needed (a forward-mode tangent is the node's to refuse).
-  bool node = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
-                                             v.requires_grad() || lam.requires_grad());
-  for (const Tensor* t : {&q, &k, &v, &lam}) node = node || torch::autograd::isFwGradDefined(*t);
-  Tensor out;
-  {
-    pybind11::gil_scoped_release no_gil;
-    if (node) {
-      out = Diff::apply(q, k, v, lam, causal, scale);
-    } else {
-      at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(q.device());
-      out = Diff::run(q, k, v, lam, causal, scale, Tensor(), Tensor());
-    }
-  }
+  Tensor out = diff_out(q, k, v, lam, causal, scale);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
 // ---------------------------------------------------------------------------
-// Cached steps, for arguments that need no conversion. These return None for anything
-// else, refusals included: decode.py then converts, or says what is wrong.
+// Differential attention and cached steps, for arguments that need no conversion. These
+// return None for anything else, refusals included: the Python then converts, or says what is
+// wrong.
 // ---------------------------------------------------------------------------
 bool plain_arg(PyObject* o, Tensor& out) {      // a Tensor itself, or None
   if (o == Py_None) return true;
@@ -428,15 +428,17 @@ bool cache_ok(const Tensor& t, const Tensor& k) {
 
 bool tracked(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-// Whether k, v [B,T,Hkv,D] are what the kernels read, on the current device, with nothing
-// for autograd or autocast to do.
-bool block_ok(const Tensor& k, const Tensor& v) {
+// Whether k, v [B,T,Hkv,D] are what the kernels read, with nothing for autocast to do.
+bool rows_ok(const Tensor& k, const Tensor& v) {
   if (!k.defined() || k.dim() != 4 || !k.is_cuda() || !kernel_type(k.scalar_type()) || !k.is_contiguous())
     return false;
   if (!dense_like(v, k, k.scalar_type(), k.sizes())) return false;
   const int64_t D = k.size(3);
-  if ((D != 32 && D != 64 && D != 128) || k.size(2) == 0) return false;
-  if (k.get_device() != c10::hip::current_device() || at::autocast::is_autocast_enabled(at::kCUDA)) return false;
+  return (D == 32 || D == 64 || D == 128) && k.size(2) != 0 && !at::autocast::is_autocast_enabled(at::kCUDA);
+}
+// ... on the current device, with nothing for autograd to do either.
+bool block_ok(const Tensor& k, const Tensor& v) {
+  if (!rows_ok(k, v) || k.get_device() != c10::hip::current_device()) return false;
   return !at::GradMode::is_enabled() || (!tracked(k) && !tracked(v));
 }
 
@@ -527,6 +529,30 @@ PyObject* py_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// diff(q, k, v, lam, scale or None, causal) -> out, or None.
+PyObject* py_diff(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, lam;
+  TORCH_CHECK_TYPE(n == 6, "diff(q, k, v, lam, scale, causal)");
+  if (!plain_arg(args[0], q) || !plain_arg(args[1], k) || !plain_arg(args[2], v) || !plain_arg(args[3], lam))
+    Py_RETURN_NONE;
+  const int causal = PyObject_IsTrue(args[5]);
+  double scale = 0.0;
+  if (args[4] != Py_None) scale = PyFloat_AsDouble(args[4]);
+  if (PyErr_Occurred()) throw python_error();
+  if (!q.defined() || q.dim() != 4 || !lam.defined() || !rows_ok(k, v)) Py_RETURN_NONE;
+  const int64_t H = q.size(2), E = k.size(3);
+  if (!dense_like(q, k, k.scalar_type(), {k.size(0), k.size(1), H, E}) || H % k.size(2) || q.numel() == 0 ||
+      !kernel_type(lam.scalar_type()) || !dense_like(lam, k, lam.scalar_type(), {H}))
+    Py_RETURN_NONE;
+  if (args[4] == Py_None) scale = std::sqrt(2.0 / static_cast<double>(E));
+  if (!std::isfinite(scale) || !(scale > 0.0)) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!fits_int(q.size(i))) Py_RETURN_NONE;
+  return THPVariable_Wrap(diff_out(q, k, v, lam, causal, scale));
+  END_HANDLE_TH_ERRORS
+}
+
 // tree_commit(k, v, cache k, cache v, lens, path, count) -> the new lens or None.
 PyObject* py_tree_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -564,6 +590,8 @@ PyMethodDef methods[] = {
      "prologue(x, weight, cos, sin, eps, out_dtype) -> out"},
     {"diff_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_diff_attn)), METH_FASTCALL,
      "diff_attn(q, k, v, lam, causal, scale) -> out"},
+    {"diff", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_diff)), METH_FASTCALL,
+     "diff(q, k, v, lam, scale, causal) -> out or None"},
     {"step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_step)), METH_FASTCALL,
      "step(q, k, v, cache_k, cache_v, lens, parents, lam, gate, causal, scale, return_lse) -> out, (out, lse) or None"},
     {"tree_commit", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_tree_commit)), METH_FASTCALL,

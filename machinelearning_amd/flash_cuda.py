@@ -639,6 +639,10 @@ def diff_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tens
 
     Raises ValueError for unsupported inputs and RuntimeError when the library cannot run.
     """
+    if _mma_ok and _f32_ok and not _python_node():       # arguments that need no conversion
+        out = _ext.diff(q, k, v, lam, scale, causal)
+        if out is not None:
+            return out
     who = "flash_cuda.diff_attn"
     dtype, scale = _check_diff(q, k, v, scale, who)
     lam = _lam_of(lam, q, who)
