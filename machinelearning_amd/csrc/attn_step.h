@@ -26,11 +26,11 @@ struct StepParams {
   const void* lam;                     // [H] map weights (two maps only)
   int lam_dtype;
   int R;                               // query rows per kv head: T * rep
-  int nsplit;                          // key splits of a unit (16-bit: workgroups in all)
-  bool direct;                         // 16-bit: a workgroup per unit
-  int min_blocks;                      // 16-bit: key blocks that a workgroup takes at least
-  float resc_th;                       // 16-bit: lazy-rescale threshold in raw score units
-  FastDiv div_rep, div_ups, div_ngrp;  // by rep; 16-bit: units per sequence, row groups
+  int nsplit;                          // workgroups
+  bool direct;                         // a workgroup per unit
+  int min_blocks;                      // key blocks that a workgroup takes at least
+  float resc_th;                       // lazy-rescale threshold in raw score units
+  FastDiv div_rep, div_ups, div_ngrp;  // by rep, units per sequence, row groups
 };
 
 constexpr int kTreeMax = 256;          // nodes of a tree: one per thread of a workgroup
