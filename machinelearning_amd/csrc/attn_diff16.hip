@@ -865,8 +865,12 @@ hipError_t diff16_fwd_t(const void* q, const void* k, const void* v, void* o, vo
   return hipGetLastError();
 }
 
-// Whether dK/dV deals its steps evenly, and how: where a workgroup per key block fills the
-// chip's slots less than twice. Fills the line's fields.
+// Whether dK/dV deals its steps evenly, and how: where the key blocks are no more than the
+// workgroups that the chip holds at once. Forward + backward, the line's us for a workgroup per
+// block's: 105 blocks of E = 32 (full) 80.6 for 106.5, 256 of E = 128 (causal rows of 8192) 1522
+// for 1915, 512 of E = 64 290 for 295 (rows of 4096) and 140 for 136 (of 1024); but 768 of E = 64
+// 230 for 211 and 149 for 137, 384 of E = 128 385 for 383, 512 of E = 128 276 for 249. Fills the
+// line's fields.
 int line_slots(int E) { return E <= 64 ? 512 : 256; }
 
 void diff16_line(DiffParams& p, int E) {
@@ -874,7 +878,7 @@ void diff16_line(DiffParams& p, int E) {
   const long long nblk = (p.S + 127) / 128, units = nblk * p.B * p.Hkv;
   const long long NT = (p.S + 63) / 64;
   const long long head = nblk * (p.group * NT + kLineSetup) - (p.causal ? p.group * nblk * (nblk - 1) : 0);
-  if (units >= 2LL * line_slots(E) || head * p.B * p.Hkv >= (1LL << 30) || p.group * NT >= (1LL << 24)) return;
+  if (units > line_slots(E) || head * p.B * p.Hkv >= (1LL << 30) || p.group * NT >= (1LL << 24)) return;
   p.line_head = (int)head;
   p.line_n = (int)(head * p.B * p.Hkv);
   const int per = (p.line_n + line_slots(E) - 1) / line_slots(E);

@@ -20,6 +20,14 @@
 //    O^T += V^T P^T from registers (attn16.h's tiles).
 //  * Masks only where a block needs one: a sequence's last cached block (rows past it read
 //    as zeros through the buffer's bound) and the active block's, one word per block.
+//  * What bounds it: the cache's bytes. The loop reads 10 bytes a cycle and CU, 5.8 TB/s over
+//    the chip (32 query rows a token, D = 128, bf16, 8 sequences of up to 8192 rows: 45 us of
+//    kernel, 34 of them the loop; finding the piece and the first loads take 6, the partials 3,
+//    and their merge in a second launch 7). Merging them in the unit's last workgroup instead
+//    took 1.5 to 19 us more a call: its release and acquire write back and drop a whole L2.
+//    One token, 32 sequences of up to 4000 rows: 48 us and a merge of 5, 6.0 TB/s. float32 at
+//    D = 128 is bound by the MFMAs of 32 rows, 8200 cycles a block and wave: 121 us for 16
+//    sequences of up to 4000 rows (61 at the memory's rate).
 #include <type_traits>
 
 #include "attn16.h"
@@ -103,8 +111,12 @@ struct Step {
   static constexpr int TILE = Tile<T, D>::BYTES; // K (or V) of a block
   static constexpr int LD = TILE / 1024;         // DMA instructions per tile
   static constexpr int IPW = 2 * LD >= NG ? 2 * LD / NG : 1;   // ... of K and V per wave
-  static constexpr int NS = NK == 4 || NK * TILE > 16384 ? 2 : 3;   // ring stages
-  static constexpr int SETUP = 16;               // what starting a unit costs, in blocks
+  // Ring stages. (A fourth instead of the third, or the next block's scores under this one's
+  // softmax: within 2%, the loop runs at the memory's rate either way.)
+  static constexpr int NS = NK == 4 || NK * TILE > 16384 ? 2 : 3;
+  // What starting a unit costs, in blocks (4, 16, 32 of them: 59.2, 55.5, 56.0 us for 8 sequences
+  // of up to 8192 rows and 32 tokens; 66.3, 64.9, 68.4 for 32 of up to 4000 and one).
+  static constexpr int SETUP = 16;
   static constexpr int RING = NK * NS * 2 * TILE;
   // The waves' float32 results, merged in LDS (the ring's bytes, after the loop).
   static constexpr bool JOIN = NK * NM > 1;
@@ -646,26 +658,29 @@ namespace {
 // us a call. 16 bits, many units: 16 sequences x 12 kv heads of D = 64, two maps, one token,
 // 300 / 1000 / 1500 rows (3, 9, 12 steps) 8.4 / 15.3 / 18.8 for 13.8 / 18.9 / 22.7; 32 x 8 of
 // D = 128, lengths drawn from 0 to 300 / 1000: 12.5 / 23.5 for 18.1 / 26.3; but 20 x 8 of up to
-// 2000 rows (16 steps) 31.0 for 28.1. Few: 24 x 2 of D = 128, 500 / 750 / 1000 rows (4, 6, 8
-// steps) 14.1 / 16.6 / 19.0 for 16.6 / 17.2 / 17.4; 6 x 2 of D = 64, 750 / 1000 / 1250 rows
-// 10.8 / 12.5 / 13.6 for 12.3 / 12.5 / 12.1. float32: 70 x 2 of D = 128, 300 / 500 rows (6, 9
-// steps) 37.4 / 51.7 for 39.9 / 50.1; 4 x 2 of D = 128, 150 / 300 rows (3, 6 steps) 22.0 / 36.0
-// for 25.6 / 27.6; of D = 64, 300 / 500 / 800 rows (3, 5, 7 steps) 14.6 / 19.9 / 25.2 for 18.2 /
-// 19.4 / 20.4; of D = 32, 500 / 800 rows 12.7 / 15.8 for 14.0 / 14.8.
+// 2000 rows (16 steps) 31.0 for 28.1. Few: 24 x 2 of D = 128, up to 400 / 600 / 800 rows (4, 5,
+// 7 steps) 12.6 / 14.1 / 16.8 for 14.3 / 14.6 / 15.0; 3 x 2 of D = 64, 600 / 800 / 1000 rows
+// (5, 7, 8 steps) 9.2 / 10.7 / 12.2 for 10.9 / 10.5 / 11.3. float32: 70 x 2 of D = 128, 300 /
+// 500 rows (6, 9 steps) 37.4 / 51.7 for 39.9 / 50.1; 3 x 2 of D = 64, 200 / 400 / 600 rows (2,
+// 4, 5 steps) 11.7 / 17.0 / 19.8 for 15.1 / 15.3 / 15.5; 4 x 2 of D = 32, 500 / 800 rows (5, 7
+// steps) 12.7 / 15.8 for 14.0 / 14.8.
 __host__ constexpr int direct_steps(bool f32, int D, long long units) {
-  if (f32) return units >= 128 ? 7 : D >= 64 ? 4 : 6;
-  return units >= 128 ? 10 : D >= 128 ? 6 : 8;
+  if (f32) return units >= 128 ? 7 : D >= 64 ? 3 : 5;
+  return units >= 128 ? 10 : D >= 128 ? 5 : 7;
 }
 
-// Workgroups of a launch: what the chip holds at once (by LDS and registers), fewer where
-// the longest batch that the cache can hold has less than min_blocks for each.
+// Workgroups of a launch: what the chip holds at once (by LDS and registers: two per CU for
+// one, 16 sequences of up to 6000 rows, D = 64, 4 / 64 query rows: 30.0 / 36.9 for 31.2 / 38.5
+// us), fewer where the longest batch that the cache can hold has less than min_blocks for each
+// (two steps; one, two, four of them: one sequence, two kv heads, up to 2000 rows 14.1, 14.0,
+// 15.8 us, up to 6000 20.1, 16.7, 17.7).
 template <typename T, int D, int MAPS, int NR, int NK>
 void step_geometry(StepParams& p) {
   using C = Step<T, D, MAPS, NR, NK>;
   constexpr int per_cu = C::LDS > 80 * 1024 || C::W == 8 ? 1 : 2;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS;
   const long long most = (long long)p.B * p.Hkv * ngrp * ((p.rows + 31) / 32 + (p.T + 31) / 32 + C::SETUP);
-  p.min_blocks = 4 * NK;
+  p.min_blocks = 2 * NK;
   p.div_ups = fast_div((unsigned)(p.Hkv * ngrp));
   p.div_ngrp = fast_div((unsigned)ngrp);
   const long long want = (most + p.min_blocks - 1) / p.min_blocks;
@@ -696,7 +711,10 @@ hipError_t step_t(const void* q, const void* kc, const void* vc, const void* kn,
 }
 
 // f(T, D, MAPS, NR, NK) for a step: row waves by the row tiles of a kv head, key groups by
-// what the ring of two stages takes (four 128-wide float32 ones would not fit).
+// what the ring of two stages takes (four 128-wide float32 ones would not fit). Against the
+// next larger form, us: one tile 64.9 for 67.1 (32 sequences, D = 128, one token) and 17.5 for
+// 19.8 (D = 64); two 44.8 for 52.9 (8 sequences of 4096 rows, D = 128, two maps, 16 tokens);
+// three or four 55.5 for 69.4 (8 sequences of up to 8192 rows, D = 128, 32 tokens).
 template <typename F>
 auto step_by_shape(int dtype, const StepParams& p, int D, bool two_maps, F f) {
   const auto by_rows = [&](auto t, auto d, auto maps) {
