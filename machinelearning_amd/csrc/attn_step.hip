@@ -20,6 +20,8 @@
 //    O^T += V^T P^T from registers (attn16.h's tiles).
 //  * Masks only where a block needs one: a sequence's last cached block (rows past it read
 //    as zeros through the buffer's bound) and the active block's, one word per block.
+//  * P^T of 16-bit inputs is rounded to their type (half a step each): the matrix
+//    instructions take 16-bit operands. Partials, statistics and sums are float32.
 //  * What bounds it: the cache's bytes. The loop reads 10 bytes a cycle and CU, 5.8 TB/s over
 //    the chip (32 query rows a token, D = 128, bf16, 8 sequences of up to 8192 rows: 45 us of
 //    kernel, 34 of them the loop; finding the piece and the first loads take 6, the partials 3,
