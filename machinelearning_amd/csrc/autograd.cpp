@@ -53,8 +53,13 @@ int code_of(const Tensor& t) {
 float* floats(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// A gradient as the kernels read it.
-Tensor dense(const Tensor& g, at::ScalarType dt) { return g.to(dt).contiguous(); }
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// A gradient as the kernels read it. (It may be a dense piece of a larger tensor's.)
+Tensor dense(const Tensor& g, at::ScalarType dt) {
+  const Tensor d = g.to(dt).contiguous();
+  return aligned16(d) ? d : d.clone();
+}
 
 // The node runs once: its gradients cannot be differentiated again
 // (torch.autograd.function.once_differentiable).
@@ -422,8 +427,7 @@ bool cache_ok(const Tensor& t, const Tensor& k) {
     return false;
   const int64_t D = k.size(3), chunk = 16 / t.element_size();
   return t.size(0) == k.size(0) && t.size(1) == k.size(2) && t.size(3) == D && t.stride(3) == 1 &&
-         t.stride(2) == D && t.stride(0) % chunk == 0 && t.stride(1) % chunk == 0 &&
-         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+         t.stride(2) == D && t.stride(0) % chunk == 0 && t.stride(1) % chunk == 0 && aligned16(t);
 }
 
 bool tracked(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -434,7 +438,7 @@ bool rows_ok(const Tensor& k, const Tensor& v) {
     return false;
   if (!dense_like(v, k, k.scalar_type(), k.sizes())) return false;
   const int64_t D = k.size(3);
-  return (D == 32 || D == 64 || D == 128) && k.size(2) != 0 && !at::autocast::is_autocast_enabled(at::kCUDA);
+  return (D == 32 || D == 64 || D == 128) && k.size(2) != 0 && aligned16(k) && aligned16(v) && !at::autocast::is_autocast_enabled(at::kCUDA);
 }
 // ... on the current device, with nothing for autograd to do either.
 bool block_ok(const Tensor& k, const Tensor& v) {
@@ -480,7 +484,7 @@ PyObject* py_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) throw python_error();
   if (!q.defined() || q.dim() != 4 || !block_ok(k, v) || ck.defined() != cv.defined()) Py_RETURN_NONE;
   const int64_t B = k.size(0), T = k.size(1), Hkv = k.size(2), D = k.size(3), H = q.size(2);
-  if (!dense_like(q, k, k.scalar_type(), {B, T, H, D}) || H % Hkv) Py_RETURN_NONE;
+  if (!dense_like(q, k, k.scalar_type(), {B, T, H, D}) || H % Hkv || !aligned16(q)) Py_RETURN_NONE;
   if (ck.defined() && (!cache_ok(ck, k) || !cache_ok(cv, k) || ck.size(2) != cv.size(2) || !fits_int(ck.size(2))))
     Py_RETURN_NONE;
   if (lens.defined() && !dense_like(lens, k, at::kInt, {B})) Py_RETURN_NONE;
@@ -542,7 +546,7 @@ PyObject* py_diff(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) throw python_error();
   if (!q.defined() || q.dim() != 4 || !lam.defined() || !rows_ok(k, v)) Py_RETURN_NONE;
   const int64_t H = q.size(2), E = k.size(3);
-  if (!dense_like(q, k, k.scalar_type(), {k.size(0), k.size(1), H, E}) || H % k.size(2) || q.numel() == 0 ||
+  if (!dense_like(q, k, k.scalar_type(), {k.size(0), k.size(1), H, E}) || H % k.size(2) || q.numel() == 0 || !aligned16(q) ||
       !kernel_type(lam.scalar_type()) || !dense_like(lam, k, lam.scalar_type(), {H}))
     Py_RETURN_NONE;
   if (args[4] == Py_None) scale = std::sqrt(2.0 / static_cast<double>(E));
@@ -562,6 +566,8 @@ PyObject* py_tree_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !plain_arg(args[4], lens) || !plain_arg(args[5], path) || !plain_arg(args[6], count))
     Py_RETURN_NONE;
   if (!block_ok(k, v) || !cache_ok(ck, k) || !cache_ok(cv, k) || ck.size(2) != cv.size(2)) Py_RETURN_NONE;
+  for (const Tensor* t : {&ck, &cv})             // sequences or heads that share their rows
+    if ((t->size(0) > 1 && t->stride(0) == 0) || (t->size(1) > 1 && t->stride(1) == 0)) Py_RETURN_NONE;
   const int64_t B = k.size(0);
   if (!path.defined() || path.dim() != 2) Py_RETURN_NONE;
   const int64_t P = path.size(1);

@@ -968,6 +968,10 @@ int mi_attn_tree_commit(const void* k_new, const void* v_new, void* k_cache, voi
   if (P < 0) return MI_ERR_SHAPE;
   if (s->B == 0) return MI_OK;
   if (!lens || !count || !lens_out || lens_out == lens) return MI_ERR_NULL;
+  // Rows that sequences or heads share cannot be written for each.
+  if (s->rows > 0 && ((s->B > 1 && (s->k_batch_stride == 0 || s->v_batch_stride == 0)) ||
+                      (s->Hkv > 1 && (s->k_head_stride == 0 || s->v_head_stride == 0))))
+    return MI_ERR_SHAPE;
   const long long elem = s->dtype == MI_F32 ? 4 : 2;
   mi::CommitParams p = {};
   p.B = s->B;

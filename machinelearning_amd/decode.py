@@ -91,7 +91,8 @@ def _shape(key: tuple):
 def _dense(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     if t.dtype != dtype:
         t = t.to(dtype)
-    return t if t.is_contiguous() else t.contiguous()
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()    # a dense piece of a larger tensor
 
 
 def _workspace(dev: torch.device, stream: int, floats: int) -> torch.Tensor:
@@ -115,7 +116,7 @@ def _cache_tensor(t, B, Hkv, D, dtype, device, who, name):
     chunk = 16 // t.element_size()
     if (t.stride(3) != 1 or t.stride(2) != D or t.stride(0) % chunk or t.stride(1) % chunk
             or t.data_ptr() % 16):
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -571,6 +572,9 @@ def tree_commit(k: torch.Tensor, v: torch.Tensor, cache: dict, path: torch.Tenso
                 or t.stride(0) % chunk or t.stride(1) % chunk or t.data_ptr() % 16):
             raise ValueError(f"{who}: cache[{name!r}] must be {dtype} on {dev} with rows {D} apart, "
                              f"16-byte aligned; got {t.dtype} on {t.device}, strides {t.stride()}")
+        if (B > 1 and t.stride(0) == 0) or (Hkv > 1 and t.stride(1) == 0):
+            raise ValueError(f"{who}: cache[{name!r}]'s sequences or heads share their rows, which "
+                             f"cannot be written (strides {t.stride()})")
     ck, cv = cache["k"], cache["v"]
     rows = int(ck.shape[2])
     if cv.shape[2] != rows:

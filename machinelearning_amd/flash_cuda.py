@@ -575,6 +575,7 @@ class _DiffAttnFn(torch.autograd.Function):
         lib = _capi.load()
         shp = ctypes.byref(_diff_shape(q, k, lam, ctx.causal, ctx.scale))
         do = do.to(q.dtype).contiguous()
+        do = do if do.data_ptr() % 16 == 0 else do.clone()
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         dlam = torch.empty_like(lam) if q.numel() else torch.zeros_like(lam)
         n = ctypes.c_longlong(0)
@@ -652,6 +653,8 @@ def diff_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tens
     q, k, v = (t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
                for t in (q, k, v))
     q, scale = _positive_scale(q, scale)
+    # (Dense pieces of larger tensors may begin anywhere.)
+    q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
     mma = dtype in MMA_DTYPES and _mma_ok
     if not mma and not _f32_ok:
         raise RuntimeError(f"float32 path unavailable ({_f32_error})")

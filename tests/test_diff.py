@@ -321,6 +321,35 @@ def test_reproducible_and_the_python_node_agrees(monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("plain_node", [False, True], ids=["cpp", "python"])
+def test_unaligned_tensors(plain_node, monkeypatch):
+    """Dense pieces of larger tensors that begin anywhere: inputs, and the gradient that a
+    concatenation hands back."""
+    if plain_node:
+        assert fc._load() is not None
+        monkeypatch.setattr(fc, "_ext", None)
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(2, 33, h, 64, generator=g).to("cuda", torch.bfloat16) for h in (4, 2, 2))
+    lam = torch.rand(4, generator=g).cuda()
+    weight = torch.randn(1 + q.numel(), generator=g).to("cuda", torch.bfloat16)
+
+    def step(shift):
+        leaves, seen = [], []
+        for t in (q, k, v):
+            leaf = torch.cat([t.new_zeros(shift), t.reshape(-1)]).requires_grad_()
+            leaves.append(leaf)
+            seen.append(leaf[shift:].view(t.shape))
+        if shift:
+            assert all(t.is_contiguous() and t.data_ptr() % 16 != 0 for t in seen)
+        w = lam.clone().requires_grad_()
+        y = fc.diff_attn(*seen, w)
+        flat = torch.cat([y.new_zeros(shift), y.reshape(-1)])      # its gradient: a shifted piece
+        grads = torch.autograd.grad(flat, leaves + [w], weight[1 - shift:])
+        return [y, grads[3]] + [t[shift:] for t in grads[:3]]
+    assert all(torch.equal(a, b) for a, b in zip(step(0), step(1)))
+
+
+@gpu
 def test_other_stream_and_graph():
     q, k, v, do, lam = (t.cuda() for t in draw(2, 260, 4, 2, 64, torch.bfloat16, seed=12))
     leaves = [t.clone().requires_grad_() for t in (q, k, v, lam)]

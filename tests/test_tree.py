@@ -171,6 +171,8 @@ def test_abi_refuses_pointers():
         assert put(**{f"a{i}": 0x1008}) == 6, i
     assert put(a7=commit[4]) == 1                                        # lens_out is lens
     assert put(P=-1) == 2
+    for shared in ("k_batch_stride", "k_head_stride", "v_batch_stride", "v_head_stride"):
+        assert put(s=step_shape(**{shared: 0})) == 2
     empty = step_shape(B=0)
     assert lib.mi_attn_step(*[None] * 12, ctypes.byref(empty), None) == 0
     assert lib.mi_attn_tree_commit(*[None] * 8, 1, ctypes.byref(empty), None) == 0
@@ -254,6 +256,8 @@ def test_refusals():
     refused("cache\\['v'\\] must be", put, k, v, {**cache, "v": cv.transpose(2, 3)}, path, count)
     refused("cache\\['v'\\] must be", put, k, v, {**cache, "v": None}, path, count)
     refused("lengths differ", put, k, v, {**cache, "v": cv[:, :, :4]}, path, count)
+    refused("share their rows", put, k, v, {**cache, "v": cv[:1].expand_as(cv)}, path, count)
+    refused("share their rows", put, k, v, {**cache, "k": ck[:, :1].expand_as(ck)}, path, count)
     assert torch.equal(cache["lens"], lens)
 
 
@@ -405,6 +409,39 @@ def test_gate_scale_strides_and_types(two):
     with torch.autocast("cuda", dtype=torch.bfloat16):
         b = dec.attn_tree(q.float().cuda(), k.cuda(), v.cuda(), cache, up.cuda(), **more)
     assert torch.equal(a, b)
+
+
+def off_by_one(t):
+    """The same values, dense, one element behind a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.reshape(-1)
+    return flat[1:].view(t.shape)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DT, ids=name)
+def test_unaligned_blocks_and_shared_caches(dtype):
+    q, k, v, ck, cv, lam = (t.cuda() for t in draw(3, 6, 4, 2, 64, 90, dtype, seed=3))
+    cache = {"k": ck, "v": cv, "lens": torch.tensor([90, 4, 31], dtype=torch.int32, device="cuda")}
+    up = draft(3, 6, 1).cuda()
+    assert off_by_one(q).is_contiguous() and off_by_one(q).data_ptr() % 16 != 0
+    for maps in (None, lam):
+        want = dec.attn_tree(q, k, v, cache, up, lam=maps)
+        assert torch.equal(dec.attn_tree(*map(off_by_one, (q, k, v)), cache, up, lam=maps), want)
+        moved = {**cache, "k": off_by_one(ck), "v": off_by_one(cv)}
+        assert torch.equal(dec.attn_tree(q, k, v, moved, up, lam=maps), want)
+    want = dec.diff_attn_cached(q, k, v, lam, {"k": ck, "v": cv}, False, True)
+    got = dec.diff_attn_cached(*map(off_by_one, (q, k, v)), lam, {"k": ck, "v": cv}, False, True)
+    assert torch.equal(got, want)
+    # One prompt's rows for every sequence of the batch.
+    one = {**cache, "k": ck[:1].expand_as(ck), "v": cv[:1].expand_as(cv)}
+    own = {**cache, "k": one["k"].contiguous(), "v": one["v"].contiguous()}
+    assert torch.equal(dec.attn_tree(q, k, v, one, up), dec.attn_tree(q, k, v, own, up))
+    a, b = ({n: t.clone() for n, t in cache.items()} for _ in range(2))
+    path = torch.tensor([[0, 2], [1, 1], [5, 0]], dtype=torch.int32, device="cuda")
+    dec.tree_commit(k, v, a, path, torch.tensor([2, 2, 1], dtype=torch.int32, device="cuda"))
+    dec.tree_commit(off_by_one(k), off_by_one(v), b, path, torch.tensor([2, 2, 1], device="cuda"))
+    assert all(torch.equal(a[n], b[n]) for n in a)
 
 
 @gpu
