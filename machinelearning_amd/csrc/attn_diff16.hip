@@ -12,11 +12,14 @@
 //
 // Rounded to the inputs' type, half a step each (2^-9 of a bf16 value, 2^-12 of fp16, on
 // average), because the matrix instructions take 16-bit operands: P_m in the forward, P_1 -
-// lam P_2 and both dS_m in the backward, and the stored P_2 v that delta and dlam come from (a
-// float32 copy would be the forward's largest write). Scores, statistics and sums are float32.
+// lam P_2 and both dS_m in the backward, and the stored out and P_2 v that delta comes from (a
+// float32 copy would be the forward's largest write). That is small beside G where a row sees
+// many keys; rows whose keys are in one tile make delta from them, and dlam is corrected by what
+// dS_2's float32 sum lacks (dq and dk of sequences of 2 or 3 rows 0.0041 -> 0.0025 off, dlam
+// 0.013 -> 0.0018, its own rounding; 2% of a step). Scores, statistics and sums are float32.
 //
 // What bounds them, at B16 S1024 H12 E64 causal | B1 S8192 H16/4 E128 causal, bf16: forward 68 |
-// 439 us, dQ 78 | 488, dK/dV 93 | 677 and a join of 12. E = 64: a wave issues a MFMA in 16
+// 439 us, dQ 80 | 500, dK/dV 93 | 677 and a join of 12. E = 64: a wave issues a MFMA in 16
 // cycles, an exponential in 8, any other VALU instruction in 4; that alone is 38, 38 and 46 us.
 // The VALUs issue in 79, 61 and 56% of the busy cycles, the rest is waits inside the waves that
 // the other two (dK/dV: one) of a SIMD do not cover, and the ends of the grid. E = 128: the MFMA
@@ -346,26 +349,12 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
     }
   }
   const float lam = load_as_float(p.lam, p.lam_dtype, h);
-  const float d2 = halves_sum(part2), d1 = fmaf(lam, d2, halves_sum(part));
+  float d2 = halves_sum(part2), d1 = fmaf(lam, d2, halves_sum(part));
   float L1 = INFINITY, L2 = INFINITY;              // log2 units; rows past S: P = 0
   const long long ridx = (long long)wi.bh * p.S + qi, plane = diff_plane(p);
   if (qi < p.S) {
-    const float a = LSE[ridx], c2 = LSE[plane + ridx];
-    L1 = a * kLog2e;
-    L2 = c2 * kLog2e;
-    if (g == 0) {
-      ws[kDelta1 * plane + ridx] = d1;
-      ws[kSeed1 * plane + ridx] = a * (-1.f / p.scale);
-      ws[kSeed2 * plane + ridx] = c2 * (-1.f / p.scale);
-      ws[kCross * plane + ridx] = lam * (d2 - d1);
-    }
-  }
-  {
-    // Rows past S contribute 0 (their dO is 0). Lanes 32 apart hold the same row.
-    float sum = d2;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-    if (lane == 0) sums[wave] = sum;
+    L1 = LSE[ridx] * kLog2e;
+    L2 = LSE[plane + ridx] * kLog2e;
   }
 
   const int t_end = ((p.causal ? min(p.S, q0 + BM) : p.S) + BN - 1) / BN;
@@ -393,7 +382,8 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
   f32x16 acc[C::NA];
 #pragma unroll
   for (int x = 0; x < C::NA; ++x) acc[x] = zero16();
-  const float c = p.scale_log2, cross = d1 - d2;
+  const float c = p.scale_log2;
+  float cross, ds2 = 0.f;                          // ds2: the lane's sum of P_2 (G - delta_2)
   const int key_hi = p.causal ? min(qi, p.S - 1) : p.S - 1;
   const int wave_key_lo_end = p.causal ? qw0 : p.S, wave_key_hi_end = p.causal ? qw0 + 31 : p.S;
 
@@ -442,6 +432,7 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
         for (int e = ks * 8; e < ks * 8 + 8; ++e) {
           s1[e] *= ga[e];
           s2[e] *= ga[e] + cross;
+          ds2 += s2[e];
         }
         f1[ks] = pack_frag<T>(s1, ks * 8);
         f2[ks] = pack_frag<T>(s2, ks * 8);
@@ -472,6 +463,47 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
   for (int i = 0; i < NS - 1; ++i)
     if (i < t_end) issue(i, i);
   __builtin_amdgcn_s_waitcnt(kWaitVm0);
+  lds_barrier();
+  // Rows of few keys: dS is a small difference of G and delta, and the stored outputs' rounding
+  // would show. Their delta_m = sum_j P_m G is made from the one key tile that they see.
+  if (tw_end == 1) {
+    const char* sK = ring[0][0];
+    const char* sV = ring[0][1];
+    float e1 = 0.f, e2 = 0.f;
+    for (int mt = 0; mt < 2; ++mt) {
+      const int kb = mt * 32, roff = mt * 32 * E * 2;
+      f32x16 s1 = zero16(), s2 = zero16(), gr = zero16();
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) {
+        const frag kf = lds_frag<T>(sK + kaddr[ds] + roff), vf = lds_frag<T>(sV + kaddr[ds] + roff);
+        if (ds < DH) s1 = M::mma(kf, qf[ds], s1);
+        else s2 = M::mma(kf, qf[ds], s2);
+        gr = M::mma(vf, dof[ds], gr);
+      }
+      const unsigned keep = keep_upto(key_hi - (kb + 4 * g));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s1[e] = fast_exp2(fmaf(s1[e], c, -L1));
+        s2[e] = fast_exp2(fmaf(s2[e], c, -L2));
+      }
+      mask_keep(s1, keep, 0.f);
+      mask_keep(s2, keep, 0.f);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        e1 = fmaf(s1[e], gr[e], e1);
+        e2 = fmaf(s2[e], gr[e], e2);
+      }
+    }
+    d1 = halves_sum(e1);
+    d2 = halves_sum(e2);
+  }
+  cross = d1 - d2;
+  if (qi < p.S && g == 0) {
+    ws[kDelta1 * plane + ridx] = d1;
+    ws[kSeed1 * plane + ridx] = LSE[ridx] * (-1.f / p.scale);
+    ws[kSeed2 * plane + ridx] = LSE[plane + ridx] * (-1.f / p.scale);
+    ws[kCross * plane + ridx] = lam * (d2 - d1);
+  }
   for (int t = 0; t < t_end; t += NS) {
     step(ic<0>{}, t);
     if (t + 1 < t_end) step(ic<1>{}, t + 1);
@@ -480,6 +512,15 @@ diff16_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K, const T* __re
     }
   }
 
+  {
+    // The block's sum of delta_2, exact though the stored P_2 v is not: a row's sum of
+    // P_2 (G - delta_2) is what delta_2 lacks, P_2's sum being 1. Rows past S add 0 (their dO
+    // and P are). Lanes 32 apart hold the same row, and half of its keys each.
+    float sum = d2 + halves_sum(ds2);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+    if (lane == 0) sums[wave] = sum;
+  }
   lds_barrier();
   if (tid == 0) ws[kPlanes * plane + (long long)wi.bh * p.nblk + wi.blk] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   // Each half's columns with their own factor, then whole rows through LDS.

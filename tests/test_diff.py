@@ -321,6 +321,33 @@ def test_reproducible_and_the_python_node_agrees(monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("S,E,causal", [(2, 64, True), (3, 64, False), (9, 128, True), (64, 32, False),
+                                        (65, 64, True), (200, 128, False), (333, 64, True)])
+def test_dlam_has_no_rounding_to_16_bits(S, E, causal, dtype):
+    """With 16-bit inputs and a float32 lam, dlam = -sum P_2 G: G's products are exact in float32
+    and its sum of E of them is off by at most E 2^-24 of sum_d |dout_d v_d| =: A; P_2 is off by
+    the score's sum (E / 2 terms), its scale and the LSE, each a few 2^-24 of numbers below 16
+    here, and the exponential's 2^-22: below 2^-18 of P_2, and the rows' sums of P_2 are as near
+    to 1. With the sums over keys and rows (S^2 <= 2^17 terms in short chains: below 2^-18) that
+    is under 2^-15 sum P_2 A."""
+    q, k, v, do, lam = (t.cuda() for t in draw(2, S, 4, 2, E, dtype, seed=S))
+    w = lam.float().requires_grad_()
+    got, = torch.autograd.grad(fc.diff_attn(q, k, v, w, causal=causal), [w], do)
+    qd, kd, vd, dd = (t.cpu().double().transpose(1, 2) for t in (q, k, v, do))
+    kd, vd = (t.repeat_interleave(2, 1) for t in (kd, vd))
+    s = qd[..., E // 2:] @ kd[..., E // 2:].transpose(2, 3).contiguous() * (2 / E) ** 0.5
+    if causal:
+        s = s.masked_fill(torch.ones(S, S).triu(1).bool(), float("-inf"))
+    p2 = torch.softmax(s, -1)
+    want = -(p2 * (dd @ vd.transpose(2, 3).contiguous())).sum((0, 2, 3))
+    bound = 2.0 ** -15 * (p2 * (dd.abs() @ vd.abs().transpose(2, 3).contiguous())).sum((0, 2, 3))
+    worst = ((got.cpu().double() - want).abs() / bound).max().item()
+    print(f"worst err/bound={worst:.3f}", flush=True)
+    assert worst <= 1.0
+
+
+@gpu
 @pytest.mark.parametrize("plain_node", [False, True], ids=["cpp", "python"])
 def test_unaligned_tensors(plain_node, monkeypatch):
     """Dense pieces of larger tensors that begin anywhere: inputs, and the gradient that a
