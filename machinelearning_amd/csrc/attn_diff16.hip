@@ -19,7 +19,7 @@
 // 0.013 -> 0.0018, its own rounding; 2% of a step). Scores, statistics and sums are float32.
 //
 // What bounds them, at B16 S1024 H12 E64 causal | B1 S8192 H16/4 E128 causal, bf16: forward 68 |
-// 439 us, dQ 80 | 500, dK/dV 93 | 677 and a join of 12. E = 64: a wave issues a MFMA in 16
+// 439 us, dQ 82 | 502, dK/dV 93 | 677 and a join of 12. E = 64: a wave issues a MFMA in 16
 // cycles, an exponential in 8, any other VALU instruction in 4; that alone is 38, 38 and 46 us.
 // The VALUs issue in 79, 61 and 56% of the busy cycles, the rest is waits inside the waves that
 // the other two (dK/dV: one) of a SIMD do not cover, and the ends of the grid. E = 128: the MFMA
