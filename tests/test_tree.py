@@ -411,6 +411,33 @@ def test_gate_scale_strides_and_types(two):
     assert torch.equal(a, b)
 
 
+@gpu
+def test_cache_past_32_bits():
+    """Rows whose byte offsets pass 32 bits (4.3 GB of keys). Keys of zero give every row the same
+    weight, so the output is the values' mean: those of the last row alone are not zero. In
+    float32 the weights' sum L + 1 is exact to 2^-24 L per addition of a few thousand partial
+    sums, and the mean is rounded to bf16: 2^-8 covers both."""
+    D, rows = 128, (1 << 24) + 104
+    L = rows - 4
+    ck = torch.zeros(1, 1, rows, D, dtype=torch.bfloat16, device="cuda")
+    cv = torch.zeros_like(ck)
+    cv[0, 0, L - 1] = torch.arange(D, device="cuda") * 2.0 ** 18
+    cv[0, 0, L:] = float("nan")
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(1, 2, h, D, device="cuda").to(torch.bfloat16) for h in (4, 1, 1))
+    want = cv[0, 0, L - 1].double() / L
+    cache = {"k": ck, "v": cv, "lens": lens}
+    up = torch.tensor([-1, -1], device="cuda")
+    for lam, share in ((None, 1.0), (torch.full((4,), 0.25, device="cuda"), 0.75)):
+        out = dec.attn_tree(q, k * 0, v * 0, cache, up, lam=lam).double()
+        assert ((out - share * want).abs() <= 2.0 ** -8 * want).all()
+    path, count = torch.tensor([[1, 0]], device="cuda"), torch.tensor([2], device="cuda")
+    dec.tree_commit(k, v, cache, path, count)
+    assert cache["lens"].item() == L + 2
+    assert torch.equal(ck[0, 0, L:L + 2], k[0, [1, 0], 0]) and torch.equal(cv[0, 0, L:L + 2], v[0, [1, 0], 0])
+    assert torch.isnan(cv[0, 0, L + 2:]).all() and not ck[0, 0, :L].any()
+
+
 def off_by_one(t):
     """The same values, dense, one element behind a 16-byte boundary."""
     flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
