@@ -11,7 +11,8 @@
 //    a unit that one fragment covers is written at once, the others' fragments go to the
 //    workspace as float32 partials (at most the first and the last of a piece are partial:
 //    two slots per workgroup) and step_combine_kernel merges them in order.
-//    A cache of few rows takes none of this: a workgroup per unit (direct_steps).
+//    A cache of few rows takes none of this, nor do sequences of one length whose units about
+//    fill the chip: a workgroup per unit (direct_steps, even_direct).
 //  * Waves. NR row waves x NM map waves x NK key groups. Up to 32 rows, each of four waves
 //    takes every fourth block (its own LDS ring, no barrier in the loop) and both maps;
 //    with more rows, a group's waves share the blocks of its ring, a row tile and a map
@@ -670,14 +671,21 @@ __host__ constexpr int direct_steps(bool f32, int D, long long units) {
   if (f32) return units >= 128 ? 7 : D >= 64 ? 3 : 5;
   return units >= 128 ? 10 : D >= 128 ? 5 : 7;
 }
+// Sequences of one length whose units come to three quarters of the compute units up to half as
+// many again: a workgroup per unit at any length. One token, us, for the line's: 192 units of
+// D = 64 (two maps) 4000 rows 42.3 for 45.7, 252 of 3000 41.0 for 44.9, 384 of 2500 49.7 for
+// 55.5; of D = 128 192 of 3000 60.2 for 66.0, 384 of 2000 83.7 for 83.3; 16 tokens, 192 of D = 64,
+// 4000 rows 42.2 for 49.5. But 128 of D = 128 47.7 for 48.1, 516 of D = 64 65.0 for 56.7.
+__host__ constexpr bool even_direct(long long units) { return units >= 192 && units <= 384; }
 
 // Workgroups of a launch: what the chip holds at once (by LDS and registers: two per CU for
 // one, 16 sequences of up to 6000 rows, D = 64, 4 / 64 query rows: 30.0 / 36.9 for 31.2 / 38.5
 // us), fewer where the longest batch that the cache can hold has less than min_blocks for each
 // (two steps; one, two, four of them: one sequence, two kv heads, up to 2000 rows 14.1, 14.0,
 // 15.8 us, up to 6000 20.1, 16.7, 17.7).
+// `even`: the sequences have one length (a workspace's size is asked for without knowing).
 template <typename T, int D, int MAPS, int NR, int NK>
-void step_geometry(StepParams& p) {
+void step_geometry(StepParams& p, bool even) {
   using C = Step<T, D, MAPS, NR, NK>;
   constexpr int per_cu = C::LDS > 80 * 1024 || C::W == 8 ? 1 : 2;
   const int ngrp = (p.R + C::ROWS - 1) / C::ROWS;
@@ -690,14 +698,15 @@ void step_geometry(StepParams& p) {
   // Short caches: a workgroup per unit, with no line to find a place in, no partials and no
   // second launch.
   const long long units = (long long)p.B * p.Hkv * ngrp;
-  p.direct = ((p.rows + 31) / 32 + (p.T + 31) / 32 + NK - 1) / NK <= direct_steps(Tile<T, D>::F32, D, units);
+  p.direct = ((p.rows + 31) / 32 + (p.T + 31) / 32 + NK - 1) / NK <= direct_steps(Tile<T, D>::F32, D, units) ||
+             (even && even_direct(units));
   if (p.direct) p.nsplit = (int)units;
 }
 
 template <typename T, int D, int MAPS, int NR, int NK>
 hipError_t step_t(const void* q, const void* kc, const void* vc, const void* kn, const void* vn, void* out,
                     float* lse, float* ws, StepParams p, hipStream_t st) {
-  step_geometry<T, D, MAPS, NR, NK>(p);
+  step_geometry<T, D, MAPS, NR, NK>(p, !p.lens);
   const auto go = [&](auto tree) {
     hipLaunchKernelGGL((step_kernel<T, D, MAPS, NR, NK, decltype(tree)::value>), dim3((unsigned)p.nsplit),
                        dim3(64 * Step<T, D, MAPS, NR, NK>::W), 0, st, (const T*)q, (const T*)kc, (const T*)vc, (const T*)kn,
@@ -745,7 +754,7 @@ long long step_workspace_floats(int dtype, const StepParams& p, int D, bool two_
     constexpr int DD = decltype(d)::value, MM = decltype(m)::value, RR = decltype(nr)::value,
                   KK = decltype(nk)::value;
     StepParams g = p;
-    step_geometry<T, DD, MM, RR, KK>(g);
+    step_geometry<T, DD, MM, RR, KK>(g, false);
     return g.direct ? 0LL : 2LL * g.nsplit * Step<T, DD, MM, RR, KK>::SLOT;
   });
 }

@@ -476,7 +476,7 @@ def test_unaligned_blocks_and_shared_caches(dtype):
 @pytest.mark.parametrize("B,T,H,Hkv,E,L,causal", [
     (4, 1, 4, 4, 64, 300, True), (2, 1, 8, 2, 128, 1, False), (3, 7, 6, 3, 32, 0, True),
     (2, 33, 4, 1, 64, 130, True), (2, 33, 4, 1, 64, 130, False), (1, 300, 2, 2, 128, 95, True),
-    (1, 70, 4, 2, 32, 1000, False)])
+    (1, 70, 4, 2, 32, 1000, False), (4, 1, 48, 48, 32, 1500, True), (4, 5, 96, 48, 32, 1301, False)])
 def test_diff_cached(B, T, H, Hkv, E, L, causal, dtype):
     q, k, v, ck, cv, lam = draw(B, T, H, Hkv, E, L, dtype, seed=L)
     cache = {"k": ck.cuda(), "v": cv.cuda()} if L else {}
